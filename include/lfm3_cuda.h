@@ -293,6 +293,129 @@ int lfm3_sample_host(const float* logits, int rows, int vocab, int ld,
                      const uint32_t* recent_count, const uint64_t* seeds,
                      uint32_t* tokens);
 
+/* ---- paged K/V cache ---------------------------------------------------------
+ * No counterpart in the reference, whose sessions own one K/V ring each
+ * (engine.cpp:55-77). These operators serve ragged batches of sequences
+ * (prompt chunks and single tokens in one call) from one pool of pages per
+ * attention layer, and shrink sequences that have grown too long. All take
+ * device pointers except the descriptors themselves, allocate nothing, keep
+ * nothing between calls and only queue work on `stream`, so they can be
+ * captured into a CUDA graph: a replay reads starts, positions, table and
+ * lengths afresh, everything else (the descriptors' numbers too) is as
+ * captured. Calls that may overlap on the GPU need workspaces of their own,
+ * two captured graphs that may be replayed at once included.
+ *
+ * A sequence's rows (one cached key and value each) are numbered from 0 in
+ * the order of its tokens; row t lies in row t % page_rows of page
+ * table[t / page_rows]. Broken tables are not fatal: where starts decrease or
+ * pass `rows`, a sequence has more than max_rows rows, a length lies outside
+ * 0 .. table_pages * page_rows or a page id that a call needs outside
+ * 0 .. pages - 1, nothing outside the buffers is touched, that sequence's
+ * results are unspecified and lfm3_cuda_take_device_error() returns 6 after
+ * the stream is synchronised. lfm3_paged_check finds the same on the host. */
+typedef struct lfm3_paged_cache {
+  uint16_t* k; /* F16 [pages][page_rows][kv_heads][dim], 16-byte aligned */
+  uint16_t* v;
+  const int32_t* table;   /* [sequences][table_stride], page ids */
+  const int32_t* lengths; /* [sequences]: rows held, a call's new rows included */
+  int32_t pages, page_rows; /* page_rows: a multiple of 16 */
+  int32_t kv_heads, dim;    /* dim: 64 or 128 */
+  int32_t sequences;        /* 0 .. 4096 */
+  int32_t table_pages;      /* entries of a table row in use (most pages of a sequence) */
+  int32_t table_stride;     /* >= table_pages */
+} lfm3_paged_cache;
+/* The new rows of a call: rows starts[s] .. starts[s + 1] - 1 of its tensors
+ * belong to sequence s (n of them, 0 allowed) and are the last n of its
+ * lengths[s] rows: the i-th is row lengths[s] - n + i. A new row whose number
+ * is negative (an idle sequence of a fixed-shape graph: length 0) is not
+ * stored, sees no key, and adds no weight. Rows of the tensors before
+ * starts[0] or from starts[sequences] on are left as they are. */
+typedef struct lfm3_paged_batch {
+  const int32_t* starts;    /* [sequences + 1] */
+  const int32_t* positions; /* [rows], or NULL: each row's own number */
+  int32_t rows;             /* rows of the tensors */
+  int32_t max_rows;         /* no sequence has more new rows (1: a decode step) */
+} lfm3_paged_batch;
+
+/* Checks host copies of the arrays the descriptors point to (k, v and
+ * positions are not read): LFM3_OK, or LFM3_ERR_INVALID and a message that
+ * names the sequence. Host only. */
+int lfm3_paged_check(const lfm3_paged_cache* cache,
+                     const lfm3_paged_batch* batch);
+
+/* Per-head RMSNorm and rotation of the new rows' queries and keys (the
+ * arithmetic of lfm3_cuda_prompt_heads over a ragged batch; a NULL norm
+ * weight leaves that norm out) with the keys and values stored in their
+ * pages, in one pass. q [rows][heads][dim], k and v [rows][kv_heads][dim] and
+ * q_out (may be q) are of `type` (LFM3_F32, LFM3_F16 or LFM3_BF16), rows
+ * `*_stride` elements apart (a multiple of 8; 16-byte aligned); arithmetic in
+ * FP32, angles position * frequencies[i] / factors[i] in FP64 (factors may be
+ * NULL), one rounding to q_out's type and to F16. */
+int lfm3_cuda_paged_heads(const lfm3_paged_cache* cache,
+                          const lfm3_paged_batch* batch, uint32_t type,
+                          const void* q, size_t q_stride, const void* k,
+                          size_t k_stride, const void* v, size_t v_stride,
+                          void* q_out, size_t q_out_stride, int heads,
+                          const float* q_norm, const float* k_norm,
+                          const float* frequencies, const float* factors,
+                          float eps, void* stream);
+
+/* Causal GQA attention of the new rows over the pages (store their keys and
+ * values first): softmax(q k / sqrt(dim)) v over the keys up to the row's own,
+ * with window > 0 the last `window` of them; times sigmoid(gate[row][head])
+ * where gate is not NULL. A row that sees no key gets 0 and lse -infinity.
+ * q, out [rows][heads][dim] and gate [rows][heads] of `type`; LFM3_F32 keeps
+ * Q and the probabilities to 22 bits (two fp16 terms each), 16-bit types
+ * round the probabilities to fp16. heads / kv_heads is any whole number up to
+ * 128. lse (may be NULL): FP32 [rows][heads], the natural logarithm of the
+ * row's sum of exp(q k / sqrt(dim)), as lfm3_cuda_paged_key_weights reads it.
+ * q_stride and out_stride as in lfm3_cuda_paged_heads; out may not overlap q.
+ * `workspace`: 256-byte aligned device memory of at least
+ * lfm3_cuda_paged_attention_workspace_bytes (of the current device; 0 for
+ * invalid descriptors), contents arbitrary before and after. */
+size_t lfm3_cuda_paged_attention_workspace_bytes(const lfm3_paged_cache* cache,
+                                                 const lfm3_paged_batch* batch,
+                                                 int heads);
+int lfm3_cuda_paged_attention(const lfm3_paged_cache* cache,
+                              const lfm3_paged_batch* batch, uint32_t type,
+                              const void* q, size_t q_stride, const void* gate,
+                              size_t gate_stride, void* out, size_t out_stride,
+                              float* lse, int heads, int window,
+                              void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* Attention weight per cached key, accumulated: weights (FP32
+ * [pages][page_rows], beside the pages) of each row of the batch's sequences
+ * gains the sum over the new rows and all heads of the probability that
+ * lfm3_cuda_paged_attention gave it, exp(q k / sqrt(dim) - lse), same
+ * visibility; rows that are new in this batch start from 0. Sequences without
+ * new rows keep their weights. Sums run in a fixed order. A query row whose
+ * lse is -infinity adds nothing. */
+size_t lfm3_cuda_paged_key_weights_workspace_bytes(
+    const lfm3_paged_cache* cache, const lfm3_paged_batch* batch, int heads);
+int lfm3_cuda_paged_key_weights(const lfm3_paged_cache* cache,
+                                const lfm3_paged_batch* batch, uint32_t type,
+                                const void* q, size_t q_stride,
+                                const float* lse, float* weights, int heads,
+                                int window, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* Eviction by accumulated weight: each sequence keeps its last `recent` rows
+ * and, of the others, those of largest weight (ties: the lower row; NaN counts
+ * as largest), `keep` rows in all (0 <= recent <= keep; sequences that hold no
+ * more keep all). Kept rows become rows 0, 1, ... in their old order: keys,
+ * values and weights move to the pages of out_table (rows of table_stride
+ * entries like table: the cache's own table, or pages that no sequence of the
+ * call uses; table_pages * page_rows >= keep). out_lengths (may be
+ * cache->lengths) gets min(length, keep); kept [sequences][keep] gets each
+ * kept row's old number (entries past the new length are left as they are).
+ * Keys keep the rotation of their old positions, so later rows go on counting
+ * positions through lfm3_paged_batch. */
+int lfm3_cuda_paged_evict(const lfm3_paged_cache* cache,
+                          const int32_t* out_table, int32_t* out_lengths,
+                          float* weights, int32_t* kept, int keep, int recent,
+                          void* stream);
+
 /* ---- engine (engine.hpp) --------------------------------------------------- */
 
 typedef struct lfm3_model lfm3_model;

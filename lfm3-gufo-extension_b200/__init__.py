@@ -112,6 +112,16 @@ def library():
         "lfm3_cuda_decode_project": ([P, I, I, P, I, P, P, P, P], I),
         "lfm3_cuda_batched_quant_gemm_fp32": ([U32, P, P, P, SZ, SZ, SZ, P], I),
         "lfm3_cuda_exact_bf16_gemm_fp32_small_batch": ([P, P, P, SZ, SZ, SZ, P], I),
+        "lfm3_paged_check": ([P, P], I),
+        "lfm3_cuda_paged_heads": ([P, P, U32, P, SZ, P, SZ, P, SZ, P, SZ, I, P,
+                                   P, P, P, F, P], I),
+        "lfm3_cuda_paged_attention_workspace_bytes": ([P, P, I], SZ),
+        "lfm3_cuda_paged_attention": ([P, P, U32, P, SZ, P, SZ, P, SZ, P, I, I,
+                                       P, SZ, P], I),
+        "lfm3_cuda_paged_key_weights_workspace_bytes": ([P, P, I], SZ),
+        "lfm3_cuda_paged_key_weights": ([P, P, U32, P, SZ, P, P, I, I, P, SZ,
+                                         P], I),
+        "lfm3_cuda_paged_evict": ([P, P, P, P, P, I, I, P], I),
         "lfm3_cuda_sample_scratch_bytes": ([I, I, I], SZ),
         "lfm3_cuda_sample": ([P, I, I, I, ctypes.POINTER(abi.Sampler), P, P,
                               P, P, P, P], I),

@@ -128,6 +128,33 @@ class StepStats(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    """lfm3_paged_cache: the K/V pages of one attention layer."""
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("pages", ctypes.c_int32),
+        ("page_rows", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("sequences", ctypes.c_int32),
+        ("table_pages", ctypes.c_int32),
+        ("table_stride", ctypes.c_int32),
+    ]
+
+
+class PagedBatch(ctypes.Structure):
+    """lfm3_paged_batch: the new rows of a call over a paged cache."""
+    _fields_ = [
+        ("starts", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("rows", ctypes.c_int32),
+        ("max_rows", ctypes.c_int32),
+    ]
+
+
 def declare_synth(lib):
     """Argument types of the lfm3_synth_* entry points (include/lfm3_synth.h)."""
     lib.lfm3_synth_default_config.argtypes = [ctypes.POINTER(Config)]

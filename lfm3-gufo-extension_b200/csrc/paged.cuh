@@ -1,0 +1,147 @@
+// Paged K/V cache operators (lfm3_cuda_paged_*): the descriptors as the
+// kernels see them, the rules every kernel reads the device tables by, and
+// the launch entry points.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/lfm3_cuda.h"
+#include "common.cuh"
+
+namespace lfm3 {
+
+constexpr int kMaxPagedSequences = 4096;
+constexpr int kMaxPagedGroup = 128;
+
+// The device arrays of lfm3_paged_cache and lfm3_paged_batch, by value.
+struct PagedTables {
+  __half* k;
+  __half* v;
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int pages, page_rows, kv_heads, sequences, table_pages, table_stride;
+  int rows, max_rows;
+};
+
+// A sequence of the batch: its new rows are tensor rows row0 .. row0 + n - 1
+// and the last n of its `length` cached rows.
+struct PagedSequence {
+  int row0, n, length;
+  bool broken;
+};
+
+// The rule on starts and lengths (the host check and every kernel): a
+// sequence whose entries are broken takes part with no rows, or no keys.
+__host__ __device__ inline PagedSequence paged_sequence(const PagedTables& t,
+                                                        int s) {
+  const int begin = t.starts[s], end = t.starts[s + 1], length = t.lengths[s];
+  PagedSequence q{begin, 0, 0, false};
+  if (begin < 0 || end < begin || end > t.rows || end - begin > t.max_rows)
+    q.broken = true;
+  else
+    q.n = end - begin;
+  if (length < 0 ||
+      int64_t(length) > int64_t(t.table_pages) * t.page_rows)
+    q.broken = true;
+  else
+    q.length = length;
+  return q;
+}
+
+// Pool row (0 .. pages * page_rows - 1) of row `row` of sequence s, or -1
+// where the page id is outside the pool. row must be inside the sequence.
+__host__ __device__ inline int paged_row(const PagedTables& t,
+                                         const int32_t* table, int s, int row) {
+  const int slot = row / t.page_rows;
+  const int page = table[size_t(s) * t.table_stride + slot];
+  return page < 0 || page >= t.pages
+             ? -1
+             : page * t.page_rows + (row - slot * t.page_rows);
+}
+
+// Element types of q, k, v, out and gate.
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ float to_float(__half v) {
+  return __half2float(v);
+}
+template <>
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __half from_float(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+struct PagedHeadsArgs {
+  PagedTables t;
+  const int32_t* positions;
+  const void *q, *k, *v;
+  void* q_out;
+  size_t ldq, ldk, ldv, ldo;
+  const float *q_norm, *k_norm, *freq, *factors;
+  int heads;
+  float eps;
+};
+cudaError_t launch_paged_heads(const PagedHeadsArgs& a, uint32_t type, int dim,
+                               cudaStream_t stream);
+
+struct PagedAttentionArgs {
+  PagedTables t;
+  const void* q;
+  const void* gate;
+  void* out;
+  float* lse;
+  size_t ldq, ldg, ldo;
+  int heads, window;
+  void* workspace;
+};
+size_t paged_attention_workspace(const PagedTables& t, int dim, int heads);
+cudaError_t launch_paged_attention(const PagedAttentionArgs& a, uint32_t type,
+                                   int dim, cudaStream_t stream);
+
+struct PagedKeyWeightsArgs {
+  PagedTables t;
+  const void* q;
+  const float* lse;
+  float* weights;
+  size_t ldq;
+  int heads, window;
+  void* workspace;
+};
+size_t paged_key_weights_workspace(const PagedTables& t, int dim, int heads);
+cudaError_t launch_paged_key_weights(const PagedKeyWeightsArgs& a,
+                                     uint32_t type, int dim,
+                                     cudaStream_t stream);
+
+struct PagedEvictArgs {
+  PagedTables t;
+  const int32_t* out_table;
+  int32_t* out_lengths;
+  float* weights;
+  int32_t* kept;
+  int keep, recent;
+};
+cudaError_t launch_paged_evict(const PagedEvictArgs& a, int dim,
+                               cudaStream_t stream);
+
+}  // namespace lfm3
