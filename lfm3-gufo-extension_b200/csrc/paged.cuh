@@ -2,6 +2,7 @@
 // kernels see them, the rules every kernel reads the device tables by, and
 // the launch entry points.
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -106,6 +107,9 @@ cudaError_t launch_paged_heads(const PagedHeadsArgs& a, uint32_t type, int dim,
                                cudaStream_t stream);
 
 struct PagedAttentionArgs {
+  // [slab of 64 dims][pool row][64], boxes of 16 rows and a whole head
+  alignas(64) CUtensorMap kmap16;
+  alignas(64) CUtensorMap vmap16;
   PagedTables t;
   const void* q;
   const void* gate;
@@ -113,8 +117,13 @@ struct PagedAttentionArgs {
   float* lse;
   size_t ldq, ldg, ldo;
   int heads, window;
+  float* decode_part;  // slots of [group][dim] outputs, then of (max, sum)
   void* workspace;
 };
+// Single-token sequences of the batch, and the slots' floats.
+cudaError_t launch_paged_decode(const PagedAttentionArgs& a, uint32_t type,
+                                int dim, cudaStream_t stream);
+size_t paged_decode_floats(int dim, int group);
 size_t paged_attention_workspace(const PagedTables& t, int dim, int heads);
 cudaError_t launch_paged_attention(const PagedAttentionArgs& a, uint32_t type,
                                    int dim, cudaStream_t stream);

@@ -2,34 +2,11 @@
 // One warp per (row, head), FP32 online softmax over the row's keys.
 #include "kernels.cuh"
 #include "paged.cuh"
+#include "paged_plan.cuh"
+#include "tensor_map.hpp"
 
 namespace lfm3 {
 namespace {
-
-// The sequence that holds tensor row r (warp-wide), false if none does.
-__device__ bool find_row(const PagedTables& t, int r, PagedSequence& out,
-                         int& index) {
-  const int lane = threadIdx.x % 32;
-  for (int s0 = 0; s0 < t.sequences; s0 += 32) {
-    PagedSequence q{0, 0, 0, true};
-    if (s0 + lane < t.sequences) {
-      q = paged_sequence(t, s0 + lane);
-      if (q.broken)
-        report_error(kErrPagedTable);
-    }
-    const unsigned any = __ballot_sync(
-        0xffffffffu, !q.broken && r >= q.row0 && r < q.row0 + q.n);
-    if (any) {
-      const int l = __ffs(any) - 1;
-      index = s0 + l;
-      out.row0 = __shfl_sync(0xffffffffu, q.row0, l);
-      out.n = __shfl_sync(0xffffffffu, q.n, l);
-      out.length = __shfl_sync(0xffffffffu, q.length, l);
-      return true;
-    }
-  }
-  return false;
-}
 
 template <typename T, int DIM>
 __global__ void __launch_bounds__(256)
@@ -42,7 +19,10 @@ __global__ void __launch_bounds__(256)
     return;
   PagedSequence s{};
   int index = 0;
-  if (!find_row(a.t, r, s, index))
+  int64_t before;
+  const auto none = [](const PagedSequence&) { return int64_t(0); };
+  if (!paged_find_row(a.t, none, r, index, s, before) ||
+      paged_single(s.n, a.heads / a.t.kv_heads))
     return;
   const int own = s.length - s.n + (r - s.row0);
   const int first = a.window ? max(0, own - a.window + 1) : 0;
@@ -88,24 +68,115 @@ __global__ void __launch_bounds__(256)
     a.lse[size_t(r) * a.heads + h] = empty ? -INFINITY : m + logf(l);
 }
 
+// Merges the slots of rows that several blocks worked on, writes the rows that
+// see no key, leaves the rest. Block = one tensor row, a warp per head at a
+// time.
+constexpr int kCombineThreads = 128;
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kCombineThreads)
+    paged_combine_kernel(const __grid_constant__ PagedAttentionArgs a) {
+  constexpr int kPer = DIM / 32;  // dimensions of a lane
+  const int r = blockIdx.x, lane = threadIdx.x % 32;
+  const int kvh = a.t.kv_heads, group = a.heads / kvh;
+  PagedSequence q{};
+  int s;
+  int64_t before;
+  const auto units = [&](const PagedSequence& x) {
+    return int64_t(decode_units(x, group, a.window));
+  };
+  const bool mine = paged_find_row(a.t, units, r, s, q, before) &&
+                    paged_single(q.n, group);
+  bool broken;
+  const int64_t total = paged_total(a.t, units, broken) * kvh;
+  const int64_t share = paged_share(total, kDecodeCtas, kDecodeMinUnits);
+  const int n = decode_units(q, group, a.window);
+  grid_dependency_wait();  // in every block: this grid ends after the last one
+  if (!mine)
+    return;
+  for (int head = threadIdx.x / 32; head < a.heads;
+       head += kCombineThreads / 32) {
+    const int h = head / group, j = head % group;
+    const int64_t first = before * kvh + int64_t(h) * n;
+    const int64_t c0 = first / share, c1 = (first + n - 1) / share;
+    if (n > 0 && c0 == c1)
+      continue;  // one block had all its keys
+    // block c's slot: its first segment unless this one begins inside c
+    const auto slot = [&](int64_t c) {
+      return 2 * c + (first > c * share ? 1 : 0);
+    };
+    const float* pm = a.decode_part + size_t(2 * kDecodeCtas) * group * DIM;
+    float top = -INFINITY;
+    for (int64_t c = c0 + lane; n > 0 && c <= c1; c += 32)
+      top = fmaxf(top, pm[(slot(c) * group + j) * 2]);
+    top = warp_max(top);
+    float l = 0, o[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      o[i] = 0;
+#pragma unroll 4
+    for (int64_t c = c0; n > 0 && c <= c1; ++c) {
+      const int64_t at = slot(c) * group + j;
+      const float2 ml = *reinterpret_cast<const float2*>(pm + at * 2);
+      const float f = ml.x == -INFINITY ? 0.0F : ex2(ml.x - top);
+      l = fmaf(ml.y, f, l);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        o[i] = fmaf(a.decode_part[at * DIM + lane + 32 * i], f, o[i]);
+    }
+    float scale = n > 0 ? 1.0F / l : 0.0F;
+    if (a.gate)
+      scale /= 1 + expf(-to_float(
+                   static_cast<const T*>(a.gate)[size_t(r) * a.ldg + head]));
+    T* out = static_cast<T*>(a.out) + size_t(r) * a.ldo + size_t(head) * DIM;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      out[lane + 32 * i] = from_float<T>(n > 0 ? o[i] * scale : 0.0F);
+    if (a.lse && lane == 0)
+      a.lse[size_t(r) * a.heads + head] =
+          n > 0 ? (top + log2f(l)) * kLn2 : -INFINITY;
+  }
+}
+
 template <typename T>
-cudaError_t launch(const PagedAttentionArgs& a, int dim, cudaStream_t stream) {
-  const int64_t items = int64_t(a.t.rows) * a.heads;
-  return launch_kernel(dim == 64 ? paged_attention_kernel<T, 64>
-                                 : paged_attention_kernel<T, 128>,
-                       dim3(unsigned((items + 7) / 8)), dim3(256), 0, stream,
-                       false, a);
+cudaError_t launch(PagedAttentionArgs a, uint32_t type, int dim,
+                   cudaStream_t stream) {
+  const int group = a.heads / a.t.kv_heads;
+  const int pool = a.t.pages * a.t.page_rows;
+  cudaError_t e;
+  if ((e = encode_pool_map(&a.kmap16, a.t.k, pool, a.t.kv_heads, dim, 16,
+                           dim / 64)) ||
+      (e = encode_pool_map(&a.vmap16, a.t.v, pool, a.t.kv_heads, dim, 16,
+                           dim / 64)))
+    return e;
+  a.decode_part = static_cast<float*>(a.workspace);
+  if (group <= kDecodeMaxGroup)
+    if ((e = launch_paged_decode(a, type, dim, stream)))
+      return e;
+  if (!paged_single(a.t.max_rows, group)) {
+    const int64_t items = int64_t(a.t.rows) * a.heads;
+    if ((e = launch_kernel(dim == 64 ? paged_attention_kernel<T, 64>
+                                     : paged_attention_kernel<T, 128>,
+                           dim3(unsigned((items + 7) / 8)), dim3(256), 0,
+                           stream, false, a)))
+      return e;
+  }
+  return launch_kernel(dim == 64 ? paged_combine_kernel<T, 64>
+                                 : paged_combine_kernel<T, 128>,
+                       dim3(a.t.rows), dim3(kCombineThreads), 0, stream, true,
+                       a);
 }
 
 }  // namespace
 
-size_t paged_attention_workspace(const PagedTables&, int, int) { return 256; }
+size_t paged_attention_workspace(const PagedTables& t, int dim, int heads) {
+  return paged_decode_floats(dim, heads / t.kv_heads) * 4 + 256;
+}
 
 cudaError_t launch_paged_attention(const PagedAttentionArgs& a, uint32_t type,
                                    int dim, cudaStream_t stream) {
-  return type == LFM3_F32   ? launch<float>(a, dim, stream)
-         : type == LFM3_F16 ? launch<__half>(a, dim, stream)
-                            : launch<__nv_bfloat16>(a, dim, stream);
+  return type == LFM3_F32   ? launch<float>(a, type, dim, stream)
+         : type == LFM3_F16 ? launch<__half>(a, type, dim, stream)
+                            : launch<__nv_bfloat16>(a, type, dim, stream);
 }
 
 }  // namespace lfm3

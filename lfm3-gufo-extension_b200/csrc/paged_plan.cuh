@@ -1,0 +1,204 @@
+// How the paged attention kernels share out a ragged batch, worked out on the
+// device from starts and lengths (the host never reads them).
+//
+// The work is one line of equal units: per sequence, per row tile, per KV
+// head, the key tiles that some row of the tile sees. Block b of a kernel
+// takes units [b per, (b + 1) per) of that line, whatever sequences they fall
+// in: every block does the same work for any mix of lengths. A stretch of one
+// (sequence, row tile, KV head) inside a block's range is a segment. A segment
+// that holds all the tiles writes the output; otherwise it leaves maxima, sums
+// and unnormalised outputs in a slot of the workspace (a block has at most two
+// such segments, its first and its last: slots 2 b and 2 b + 1), and the
+// combine kernel, which finds the same places by the same rules, merges them
+// in key order.
+#pragma once
+#include "paged.cuh"
+
+namespace lfm3 {
+
+// Single-token rows: keys in blocks of 16, one row tile per sequence.
+constexpr int kDecodeKeys = 16;
+constexpr int kDecodeCtas = 296;      // two per SM
+constexpr int kDecodeMinUnits = 8;    // a block takes at least 128 keys
+constexpr int kDecodeMaxGroup = 16;   // more heads per KV head: chunk kernel
+// Chunks: tiles of 128 keys against pairs of 128-row tiles.
+constexpr int kChunkKeys = 128;
+constexpr int kChunkCtas = 148;       // one per SM
+constexpr int kChunkRows = 128;       // (query, head of the group) rows, M
+
+__host__ __device__ inline bool paged_single(int n, int group) {
+  return n == 1 && group <= kDecodeMaxGroup;
+}
+// Queries of a row tile (its rows are query-major: query i / group).
+__host__ __device__ inline int chunk_queries(int group) {
+  return kChunkRows / group;
+}
+
+// First and last key that rows qlo .. qhi (of the sequence's new rows) see;
+// last < first where they see none.
+__host__ __device__ inline void paged_key_range(const PagedSequence& q,
+                                                int window, int qlo, int qhi,
+                                                int& first, int& last) {
+  const int base = q.length - q.n;
+  last = base + qhi;
+  first = window > 0 && base + qlo >= window ? base + qlo - window + 1 : 0;
+}
+
+// Key units of a row tile (rows qlo .. qhi), from unit `lo`.
+__host__ __device__ inline int paged_units(const PagedSequence& q, int window,
+                                           int qlo, int qhi, int keys,
+                                           int& lo) {
+  int first, last;
+  paged_key_range(q, window, qlo, qhi, first, last);
+  lo = first / keys;
+  return last < first ? 0 : last / keys - lo + 1;
+}
+
+// Key units of a single-token sequence (0 for every other).
+__device__ inline int decode_units(const PagedSequence& q, int group,
+                                   int window) {
+  int lo;
+  return paged_single(q.n, group)
+             ? paged_units(q, window, 0, 0, kDecodeKeys, lo)
+             : 0;
+}
+
+// Pairs of row tiles of a chunk (0 for single tokens), and a pair's tiles.
+__device__ inline int chunk_pairs(const PagedSequence& q, int group) {
+  if (paged_single(q.n, group))
+    return 0;
+  const int queries = 2 * chunk_queries(group);
+  return (q.n + queries - 1) / queries;
+}
+__device__ inline int chunk_units(const PagedSequence& q, int group,
+                                  int window, int pair, int& lo) {
+  const int queries = 2 * chunk_queries(group);
+  return paged_units(q, window, pair * queries,
+                     min(q.n, (pair + 1) * queries) - 1, kChunkKeys, lo);
+}
+__device__ inline int64_t chunk_sequence_units(const PagedSequence& q,
+                                               int group, int window) {
+  const int pairs = chunk_pairs(q, group);
+  int64_t sum = 0;
+  int lo;
+  for (int p = 0; p < pairs; ++p)
+    sum += chunk_units(q, group, window, p, lo);
+  return sum;
+}
+
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Sum of units(sequence) over the batch, and whether a sequence is broken
+// (warp-wide).
+template <typename Units>
+__device__ int64_t paged_total(const PagedTables& t, Units units,
+                               bool& broken) {
+  int64_t sum = 0;
+  broken = false;
+  for (int s = threadIdx.x % 32; s < t.sequences; s += 32) {
+    const PagedSequence q = paged_sequence(t, s);
+    broken |= q.broken;
+    sum += units(q);
+  }
+  return warp_sum64(sum);
+}
+
+// The sequence that holds unit `at` of the line of units(sequence), its
+// numbers, and the units before it (warp-wide). False past the end.
+template <typename Units>
+__device__ bool paged_find(const PagedTables& t, Units units, int64_t at,
+                           int& s, PagedSequence& q, int64_t& before) {
+  const int lane = threadIdx.x % 32;
+  int64_t sum = 0;
+  for (int s0 = 0; s0 < t.sequences; s0 += 32) {
+    PagedSequence mine{0, 0, 0, true};
+    int64_t u = 0;
+    if (s0 + lane < t.sequences) {
+      mine = paged_sequence(t, s0 + lane);
+      u = units(mine);
+    }
+    int64_t inc = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o)
+        inc += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, sum + inc > at);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      s = s0 + l;
+      q.row0 = __shfl_sync(0xffffffffu, mine.row0, l);
+      q.n = __shfl_sync(0xffffffffu, mine.n, l);
+      q.length = __shfl_sync(0xffffffffu, mine.length, l);
+      q.broken = false;
+      before = sum + __shfl_sync(0xffffffffu, inc - u, l);
+      return true;
+    }
+    sum += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return false;
+}
+
+// The same for the sequence that holds tensor row r.
+template <typename Units>
+__device__ bool paged_find_row(const PagedTables& t, Units units, int r,
+                               int& s, PagedSequence& q, int64_t& before) {
+  const int lane = threadIdx.x % 32;
+  int64_t sum = 0;
+  for (int s0 = 0; s0 < t.sequences; s0 += 32) {
+    PagedSequence mine{0, 0, 0, true};
+    if (s0 + lane < t.sequences)
+      mine = paged_sequence(t, s0 + lane);
+    const int64_t u = units(mine);
+    const unsigned hit = __ballot_sync(
+        0xffffffffu, mine.n > 0 && r >= mine.row0 && r < mine.row0 + mine.n);
+    if (!hit) {
+      sum += warp_sum64(u);
+      continue;
+    }
+    const int l = __ffs(hit) - 1;
+    s = s0 + l;
+    q.row0 = __shfl_sync(0xffffffffu, mine.row0, l);
+    q.n = __shfl_sync(0xffffffffu, mine.n, l);
+    q.length = __shfl_sync(0xffffffffu, mine.length, l);
+    q.broken = false;
+    before = sum + warp_sum64(lane < l ? u : 0);
+    return true;
+  }
+  return false;
+}
+
+// Units per block for a line of `total` units over `ctas` blocks.
+__device__ __forceinline__ int64_t paged_share(int64_t total, int ctas,
+                                               int least) {
+  return max((total + ctas - 1) / ctas, int64_t(least));
+}
+
+// ---- numbers of the softmax ---------------------------------------------------
+// Scores are kept in base 2: x = (q k) rsqrt(dim) log2 e.
+constexpr float kLog2e = 1.44269504088896341F;
+constexpr float kLn2 = 0.693147180559945309F;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The power of two that brings a row's largest magnitude into [2^14, 2^15),
+// so that its fp16 terms neither overflow nor lose bits (1 for rows of zeros
+// or with values that are not finite).
+__device__ __forceinline__ float row_scale(float top) {
+  const int e = int(__float_as_uint(top) >> 23);
+  if (!(top > 0) || e == 255)
+    return 1.0F;
+  return __uint_as_float(uint32_t(min(127 + 14 - (e - 127), 254)) << 23);
+}
+
+}  // namespace lfm3

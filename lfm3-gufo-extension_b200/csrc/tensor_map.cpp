@@ -73,6 +73,28 @@ cudaError_t encode_activation_map(CUtensorMap* map, const void* base, int rows,
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t encode_pool_map(CUtensorMap* map, const void* base, int rows,
+                            int heads, int dim, int box_rows, int box_slabs) {
+  const EncodeTiled encode = Encoder();
+  if (!encode)
+    return cudaErrorNotSupported;
+  if (rows < 1 || heads < 1 || dim % 64 || box_rows < 8 || box_rows % 8 ||
+      box_rows > 256 || box_slabs < 1 || box_slabs > dim / 64 ||
+      reinterpret_cast<uintptr_t>(base) % 16)
+    return cudaErrorInvalidValue;
+  const cuuint64_t pitch = cuuint64_t(heads) * dim * 2;
+  const cuuint64_t dims[3] = {64, cuuint64_t(rows), cuuint64_t(heads) * dim / 64};
+  const cuuint64_t strides[2] = {pitch, 128};
+  const cuuint32_t box[3] = {64, cuuint32_t(box_rows), cuuint32_t(box_slabs)};
+  const cuuint32_t element_strides[3] = {1, 1, 1};
+  const CUresult r = encode(
+      map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims,
+      strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 namespace {
 // kind, base, size, rows, box width, box rows
 using MapKey = std::tuple<int, const void*, size_t, int, int, int>;

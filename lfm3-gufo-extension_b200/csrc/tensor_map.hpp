@@ -23,8 +23,15 @@ cudaError_t encode_q8_rows(CUtensorMap* map, const void* base, size_t row_bytes,
 cudaError_t encode_activation_map(CUtensorMap* map, const void* base, int rows,
                                   int cols, int box_rows, int box_cols);
 
-// The same maps from a process-wide cache keyed by every encode argument
-// (a hit is exactly the map the encoder would write).
+// Encodes a map over a pool of fp16 rows [rows][heads * dim] (dim a multiple
+// of 64) as [heads * dim / 64][rows][64] with boxes of box_slabs x box_rows x
+// 64 and the 128-byte swizzle: one copy lands box_rows of a head as dim / 64
+// (box_slabs) slabs of 128-byte rows. Box coordinates: 0, row, slab.
+cudaError_t encode_pool_map(CUtensorMap* map, const void* base, int rows,
+                            int heads, int dim, int box_rows, int box_slabs);
+
+// The weight and activation maps from a process-wide cache keyed by every
+// encode argument (a hit is exactly the map the encoder would write).
 cudaError_t cached_q8_rows(CUtensorMap* map, const void* base, size_t row_bytes,
                            int rows, int box_bytes, int box_rows);
 cudaError_t cached_activation_map(CUtensorMap* map, const void* base, int rows,
