@@ -28,8 +28,8 @@ SOURCES = [
     "abi.cu", "attention_decode.cu", "attention_prompt.cu",
     "attention_prompt_tc.cu", "conv.cu",
     "device_error.cu", "engine.cpp", "noalloc.cu", "norm.cu",
-    "paged_abi.cu", "paged_attention.cu", "paged_decode.cu", "paged_evict.cu",
-    "paged_heads.cu",
+    "paged_abi.cu", "paged_attention.cu", "paged_chunk.cu", "paged_decode.cu",
+    "paged_evict.cu", "paged_heads.cu",
     "paged_key_weights.cu", "q8_decode.cu",
     "q8_gemv.cu",
     "q8_prefill.cu", "sampling.cu", "scheduler.cpp",

@@ -110,6 +110,10 @@ struct PagedAttentionArgs {
   // [slab of 64 dims][pool row][64], boxes of 16 rows and a whole head
   alignas(64) CUtensorMap kmap16;
   alignas(64) CUtensorMap vmap16;
+  // the same pools, boxes of box_rows rows of one slab
+  alignas(64) CUtensorMap kmap;
+  alignas(64) CUtensorMap vmap;
+  int box_rows;
   PagedTables t;
   const void* q;
   const void* gate;
@@ -118,12 +122,17 @@ struct PagedAttentionArgs {
   size_t ldq, ldg, ldo;
   int heads, window;
   float* decode_part;  // slots of [group][dim] outputs, then of (max, sum)
+  float* chunk_part;   // slots of [dim / 4][256 rows][4], then of (max, sum)
   void* workspace;
 };
 // Single-token sequences of the batch, and the slots' floats.
 cudaError_t launch_paged_decode(const PagedAttentionArgs& a, uint32_t type,
                                 int dim, cudaStream_t stream);
 size_t paged_decode_floats(int dim, int group);
+// The other sequences (chunks, and wide groups), and the slots' floats.
+cudaError_t launch_paged_chunk(const PagedAttentionArgs& a, uint32_t type,
+                               int dim, cudaStream_t stream);
+size_t paged_chunk_floats(int dim);
 size_t paged_attention_workspace(const PagedTables& t, int dim, int heads);
 cudaError_t launch_paged_attention(const PagedAttentionArgs& a, uint32_t type,
                                    int dim, cudaStream_t stream);

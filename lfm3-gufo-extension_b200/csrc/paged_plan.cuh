@@ -24,6 +24,7 @@ constexpr int kDecodeMaxGroup = 16;   // more heads per KV head: chunk kernel
 // Chunks: tiles of 128 keys against pairs of 128-row tiles.
 constexpr int kChunkKeys = 128;
 constexpr int kChunkCtas = 148;       // one per SM
+constexpr int kChunkMinUnits = 1;
 constexpr int kChunkRows = 128;       // (query, head of the group) rows, M
 
 __host__ __device__ inline bool paged_single(int n, int group) {
@@ -145,7 +146,57 @@ __device__ bool paged_find(const PagedTables& t, Units units, int64_t at,
   return false;
 }
 
-// The same for the sequence that holds tensor row r.
+// One block's next piece of the chunks' line: units u0 .. u0 + count - 1 (of
+// n_units, the first of them key tile `lo_unit`) of a pair of row tiles and a
+// KV head.
+struct ChunkSegment {
+  PagedSequence q;
+  int seq, pair, h;
+  int n_units, lo_unit, u0, count;
+};
+// The segment at unit `at` of a range that ends at `end` (warp-wide).
+__device__ inline bool chunk_segment(const PagedTables& t, int group,
+                                     int window, int64_t at, int64_t end,
+                                     ChunkSegment& g) {
+  const int lane = threadIdx.x % 32, kvh = t.kv_heads;
+  const auto units = [&](const PagedSequence& q) {
+    return chunk_sequence_units(q, group, window);
+  };
+  int64_t before;
+  if (at >= end || !paged_find(t, units, at / kvh, g.seq, g.q, before))
+    return false;
+  const int pairs = chunk_pairs(g.q, group);
+  int64_t rel = at - before * kvh;
+  for (int p0 = 0; p0 < pairs; p0 += 32) {
+    int lo = 0;
+    const int64_t mine =
+        p0 + lane < pairs
+            ? int64_t(chunk_units(g.q, group, window, p0 + lane, lo)) * kvh
+            : 0;
+    int64_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o)
+        inc += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, inc > rel);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      rel -= __shfl_sync(0xffffffffu, inc - mine, l);
+      g.pair = p0 + l;
+      g.n_units = chunk_units(g.q, group, window, g.pair, g.lo_unit);
+      g.h = int(rel / g.n_units);
+      g.u0 = int(rel % g.n_units);
+      g.count = int(min(int64_t(g.n_units - g.u0), end - at));
+      return true;
+    }
+    rel -= __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return false;
+}
+
+// paged_find for the sequence that holds tensor row r.
 template <typename Units>
 __device__ bool paged_find_row(const PagedTables& t, Units units, int r,
                                int& s, PagedSequence& q, int64_t& before) {

@@ -1,5 +1,5 @@
-// tcgen05 building blocks of the prompt attention kernel: shared-memory
-// operand descriptors of the 64-byte-swizzled layouts TMA writes,
+// tcgen05 building blocks of the prompt and paged attention kernels:
+// shared-memory operand descriptors of the swizzled layouts TMA writes,
 // instruction descriptors of kind::f16, MMA issue and commit, tensor-memory
 // allocation, loads and stores.
 #pragma once
@@ -39,6 +39,30 @@ __device__ __forceinline__ uint64_t sw64_mn_desc(const void* p,
          (uint64_t(4) << 61);
 }
 
+// The same for 128-byte rows (64 fp16) with the 128-byte swizzle
+// (CU_TENSOR_MAP_SWIZZLE_128B): 8-row groups 1024 bytes apart; tiles start on
+// 1024-byte boundaries.
+__device__ __forceinline__ uint32_t sw128_offset(int row, int piece) {
+  return uint32_t(row * 128 + ((piece ^ (row & 7)) << 4));
+}
+// K-major: adding 2 advances K by 16 elements.
+__device__ __forceinline__ uint64_t sw128_desc(const void* p) {
+  const uint32_t addr = smem_addr(p);
+  return uint64_t((addr >> 4) & 0x3FFF) | (uint64_t(1) << 16) |
+         (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+// MN-major, the 64-element blocks of M (N) `block_bytes` apart: adding 128
+// advances K by 16 rows (2048 bytes).
+__device__ __forceinline__ uint64_t sw128_mn_desc(const void* p,
+                                                  uint32_t block_bytes) {
+  const uint32_t addr = smem_addr(p);
+  return uint64_t((addr >> 4) & 0x3FFF) |
+         (uint64_t((block_bytes >> 4) & 0x3FFF) << 16) |
+         (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+
 // Instruction descriptor of kind::f16: A and B fp16 K-major, D fp32, M x N.
 // b_mn_major reads B (N x K) from an MN-major tile instead.
 constexpr uint32_t f16_idesc(int m, int n, bool b_mn_major = false) {
@@ -62,6 +86,19 @@ __device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t a, uint64_t b,
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
           d_tmem),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// The same with A in tensor memory: lane = row, each 32-bit column two
+// consecutive K elements (adding 8 advances K by 16).
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem,
+                                       uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
+          d_tmem),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
