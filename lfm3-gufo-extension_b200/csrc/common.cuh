@@ -158,6 +158,13 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const void* map, int x0,
       : "memory");
 }
 
+// Asks for a tensor map (a __grid_constant__ parameter) ahead of its first use.
+__device__ __forceinline__ void prefetch_map(const void* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(
+                   reinterpret_cast<uint64_t>(map))
+               : "memory");
+}
+
 // ---- programmatic dependent launch ------------------------------------------
 // Work before grid_dependency_wait() may only touch data that no earlier
 // kernel in the stream writes (weights); everything else comes after it.

@@ -114,6 +114,9 @@ struct PagedAttentionArgs {
   alignas(64) CUtensorMap kmap;
   alignas(64) CUtensorMap vmap;
   int box_rows;
+  // the chunk kernel was launched behind the decode kernel of the same call,
+  // which waited for the work before it
+  bool behind_decode;
   PagedTables t;
   const void* q;
   const void* gate;
@@ -121,8 +124,10 @@ struct PagedAttentionArgs {
   float* lse;
   size_t ldq, ldg, ldo;
   int heads, window;
-  float* decode_part;  // slots of [group][dim] outputs, then of (max, sum)
-  float* chunk_part;   // slots of [dim / 4][256 rows][4], then of (max, sum)
+  // slots of [group][dim] outputs, then of (max, sum), then the records
+  float* decode_part;
+  // slots of [dim / 4][256 rows][4], then of (max, sum), then the records
+  float* chunk_part;
   void* workspace;
 };
 // Single-token sequences of the batch, and the slots' floats.

@@ -11,117 +11,145 @@
 namespace lfm3 {
 namespace {
 
-// Merges the slots of rows that several blocks worked on, writes the rows that
-// see no key, leaves the rest. Block = one tensor row, a warp per head at a
-// time.
+// Merges the stretches that several blocks shared, one record a time: blocks
+// 0 .. 295 (with `decode`) a single token's G heads, then eight blocks a chunk
+// record, 32 of its 256 rows each. Slots add up in key order.
 constexpr int kCombineThreads = 128;
+constexpr int kCombineRows = 32;
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kCombineThreads)
-    paged_combine_kernel(const __grid_constant__ PagedAttentionArgs a) {
-  constexpr int kPer = DIM / 32;  // dimensions of a lane
-  const int r = blockIdx.x, lane = threadIdx.x % 32;
+    paged_combine_kernel(const __grid_constant__ PagedAttentionArgs a,
+                         int decode) {
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int kvh = a.t.kv_heads, group = a.heads / kvh;
-  PagedSequence q{};
-  int s;
-  int64_t before = 0, total = 0, share = 0, first_unit = 0;
-  int n = 0;       // key units of the row's tile and KV head
-  int trow = 0;    // chunk: the row's place in its pair of row tiles
-  bool broken, single = false;
-  const auto decode = [&](const PagedSequence& x) {
-    return int64_t(decode_units(x, group, a.window));
-  };
-  const auto chunk = [&](const PagedSequence& x) {
-    return chunk_sequence_units(x, group, a.window);
-  };
-  bool mine = paged_find_row(a.t, decode, r, s, q, before);
-  if (mine && paged_single(q.n, group)) {
-    single = true;
-    n = decode_units(q, group, a.window);
-    total = paged_total(a.t, decode, broken) * kvh;
-    share = paged_share(total, kDecodeCtas, kDecodeMinUnits);
-    first_unit = before * kvh;
-  } else if (mine) {
-    mine = paged_find_row(a.t, chunk, r, s, q, before);
-    const int queries = 2 * chunk_queries(group), i = r - q.row0;
-    int lo;
-    for (int p = 0; p < i / queries; ++p)
-      before += chunk_units(q, group, a.window, p, lo);
-    n = chunk_units(q, group, a.window, i / queries, lo);
-    trow = i % queries / (queries / 2) * kChunkRows +
-           i % (queries / 2) * group;
-    total = paged_total(a.t, chunk, broken) * kvh;
-    share = paged_share(total, kChunkCtas, kChunkMinUnits);
-    first_unit = before * kvh;
-  }
-  grid_dependency_wait();  // in every block: this grid ends after the last one
-  if (!mine)
-    return;
+  __shared__ float tile[kCombineRows][DIM + 4];
+  __shared__ float4 row_scales[kCombineRows];
+  allow_dependents();
+  grid_dependency_wait();
+  const bool single = blockIdx.x < decode;
+  const int chunk = (blockIdx.x - decode) / (2 * kChunkRows / kCombineRows);
   const float* part = single ? a.decode_part : a.chunk_part;
-  const float* pm =
-      part + (single ? size_t(2 * kDecodeCtas) * group * DIM
-                     : size_t(2 * kChunkCtas) * 2 * kChunkRows * DIM);
-  for (int head = threadIdx.x / 32; head < a.heads;
-       head += kCombineThreads / 32) {
-    const int h = head / group, j = head % group;
-    const int64_t first = first_unit + int64_t(h) * n;
-    const int64_t c0 = first / share, c1 = (first + n - 1) / share;
-    if (n > 0 && c0 == c1)
-      continue;  // one block had all its keys
-    // block c's slot: its first segment unless this one begins inside c
-    const auto slot = [&](int64_t c) {
-      return 2 * c + (first > c * share ? 1 : 0);
-    };
-    // its entry of (max, sum), and this lane's four output values
-    const auto entry = [&](int64_t c) {
-      return single ? slot(c) * group + j
-                    : slot(c) * (2 * kChunkRows) + trow + j;
-    };
-    const auto values = [&](int64_t c) {
-      return single ? part + entry(c) * DIM + lane * 4
-                    : part + slot(c) * (2 * kChunkRows) * DIM +
-                          (lane * (2 * kChunkRows) + trow + j) * 4;
-    };
-    float top = -INFINITY;
-    for (int64_t c = c0 + lane; n > 0 && c <= c1; c += 32)
-      top = fmaxf(top, pm[entry(c) * 2]);
-    top = warp_max(top);
-    float l = 0, o[4] = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int64_t c = c0; n > 0 && c <= c1; ++c) {
-      const float2 ml = *reinterpret_cast<const float2*>(pm + entry(c) * 2);
-      float4 v = make_float4(0, 0, 0, 0);
-      if (lane < DIM / 4)
-        v = *reinterpret_cast<const float4*>(values(c));
-      if (ml.x == -INFINITY && ml.y == 0)
-        continue;  // no visible key there
-      const float f = ml.x == -INFINITY ? 1.0F : ex2(ml.x - top);
-      l = fmaf(ml.y, f, l);
-      o[0] = fmaf(v.x, f, o[0]);
-      o[1] = fmaf(v.y, f, o[1]);
-      o[2] = fmaf(v.z, f, o[2]);
-      o[3] = fmaf(v.w, f, o[3]);
+  const int rows = single ? group : 2 * kChunkRows;  // of a slot
+  const int slots = 2 * (single ? kDecodeCtas : kChunkCtas);
+  const float2* pm =
+      reinterpret_cast<const float2*>(part + size_t(slots) * rows * DIM);
+  const PagedRecord rec = reinterpret_cast<const PagedRecord*>(
+      pm + size_t(slots) * rows)[single ? blockIdx.x : chunk];
+  if (rec.parts == 0)
+    return;
+  // rows of the slot this block merges
+  const int first = single ? 0
+                           : (blockIdx.x - decode) %
+                                 (2 * kChunkRows / kCombineRows) * kCombineRows;
+  const int count = single ? group : kCombineRows;
+  // tensor row and head of slot row i
+  const int QB = chunk_queries(group);
+  const auto place = [&](int i, int& row, int& head) {
+    if (single) {
+      row = rec.row0;
+      head = rec.h * group + i;
+      return true;
     }
-    const bool empty = l == 0;
-    float scale = empty ? 0.0F : 1.0F / l;
-    if (a.gate)
-      scale /= 1 + expf(-to_float(
-                   static_cast<const T*>(a.gate)[size_t(r) * a.ldg + head]));
-    T* out = static_cast<T*>(a.out) + size_t(r) * a.ldo + size_t(head) * DIM;
-    if (lane < DIM / 4) {
-      alignas(16) T y[4];
+    const int t = i % kChunkRows;
+    const int qi = rec.pair * 2 * QB + i / kChunkRows * QB + t / group;
+    row = rec.row0 + qi;
+    head = rec.h * group + t % group;
+    return t < QB * group && qi < rec.n;
+  };
+  // ---- a row's maximum, sum and factor: eight threads a row
+  for (int i0 = 0; i0 < count; i0 += kCombineThreads / 8) {
+    const int i = i0 + tid / 8, sub = tid % 8;
+    float top = -INFINITY, l = 0;
+    if (i < count)
+      for (int p = sub; p < rec.parts; p += 8) {
+        const float2 ml = pm[record_slot(rec, p) * rows + first + i];
+        const float m = fmaxf(top, ml.x);
+        // (a sum without a maximum is 0, or NaN, which has to stay)
+        l = (top == -INFINITY ? l : l * ex2(top - m)) +
+            (ml.x == -INFINITY ? ml.y : ml.y * ex2(ml.x - m));
+        top = m;
+      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        y[i] = from_float<T>(empty ? 0.0F : o[i] * scale);
-      if constexpr (sizeof(T) == 4)
-        *reinterpret_cast<uint4*>(out + lane * 4) =
-            *reinterpret_cast<const uint4*>(y);
-      else
-        *reinterpret_cast<uint2*>(out + lane * 4) =
-            *reinterpret_cast<const uint2*>(y);
+    for (int o = 4; o; o >>= 1) {
+      const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
+      const float l2 = __shfl_xor_sync(0xffffffffu, l, o);
+      const float m = fmaxf(top, t2);
+      const bool low = (tid & o) == 0;  // both lanes add in the same order
+      const float x = top == -INFINITY ? l : l * ex2(top - m);
+      const float y = t2 == -INFINITY ? l2 : l2 * ex2(t2 - m);
+      l = low ? x + y : y + x;
+      top = m;
     }
-    if (a.lse && lane == 0)
-      a.lse[size_t(r) * a.heads + head] =
-          empty ? -INFINITY : (top + log2f(l)) * kLn2;
+    if (i < count && sub == 0) {
+      int row, head;
+      float scale = 0;
+      if (place(first + i, row, head)) {
+        scale = l == 0 ? 0.0F : 1.0F / l;
+        if (a.gate)
+          scale /= 1 + expf(-to_float(static_cast<const T*>(
+                           a.gate)[size_t(row) * a.ldg + head]));
+        if (a.lse)
+          a.lse[size_t(row) * a.heads + head] =
+              l == 0 ? -INFINITY : (top + log2f(l)) * kLn2;
+      }
+      row_scales[i] = make_float4(top, scale, 0, 0);
+    }
+  }
+  __syncthreads();
+  // ---- the outputs: chunk slots lie [dim / 4][row][4] (lane = row), single
+  // ones [row][dim] (lane = four dimensions)
+  constexpr int kQuads = DIM / 4;
+  for (int u = warp; u < (single ? count : kQuads);
+       u += kCombineThreads / 32) {
+    const int i = single ? u : lane, d4 = single ? lane : u;
+    if (d4 >= kQuads)
+      continue;
+    const float top = row_scales[i].x;
+    const size_t step = size_t(rows) * DIM;
+    const float* src = part + (single ? size_t(i) * DIM + d4 * 4
+                                      : (size_t(d4) * rows + first + i) * 4);
+    float4 o = make_float4(0, 0, 0, 0);
+    for (int p0 = 0; p0 < rec.parts; p0 += 4) {
+      float4 v[4];
+      float f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int sl = record_slot(rec, min(p0 + k, rec.parts - 1));
+        v[k] = *reinterpret_cast<const float4*>(src + sl * step);
+        const float m = pm[sl * rows + first + i].x;
+        f[k] = p0 + k >= rec.parts ? 0.0F : m == -INFINITY ? 1.0F
+                                                           : ex2(m - top);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (p0 + k >= rec.parts)
+          break;
+        o.x = fmaf(v[k].x, f[k], o.x);
+        o.y = fmaf(v[k].y, f[k], o.y);
+        o.z = fmaf(v[k].z, f[k], o.z);
+        o.w = fmaf(v[k].w, f[k], o.w);
+      }
+    }
+    const float scale = row_scales[i].y;
+    *reinterpret_cast<float4*>(&tile[i][d4 * 4]) =
+        make_float4(o.x * scale, o.y * scale, o.z * scale, o.w * scale);
+  }
+  __syncthreads();
+  for (int e = tid; e < count * kQuads; e += kCombineThreads) {
+    const int i = e / kQuads, d4 = e % kQuads;
+    int row, head;
+    if (!place(first + i, row, head))
+      continue;
+    const float4 y = *reinterpret_cast<const float4*>(&tile[i][d4 * 4]);
+    T* out = static_cast<T*>(a.out) + size_t(row) * a.ldo +
+             size_t(head) * DIM + d4 * 4;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(out) = y;
+    } else {
+      alignas(8) T z[4] = {from_float<T>(y.x), from_float<T>(y.y),
+                           from_float<T>(y.z), from_float<T>(y.w)};
+      *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(z);
+    }
   }
 }
 
@@ -142,6 +170,7 @@ cudaError_t launch(PagedAttentionArgs a, uint32_t type, int dim,
       return e;
   }
   if (!paged_single(a.t.max_rows, group)) {
+    a.behind_decode = group <= kDecodeMaxGroup;
     // the largest box that never crosses a page
     a.box_rows = std::min(a.t.page_rows & -a.t.page_rows, kChunkKeys);
     if ((e = encode_pool_map(&a.kmap, a.t.k, pool, a.t.kv_heads, dim,
@@ -151,10 +180,15 @@ cudaError_t launch(PagedAttentionArgs a, uint32_t type, int dim,
         (e = launch_paged_chunk(a, type, dim, stream)))
       return e;
   }
+  const int decode = group <= kDecodeMaxGroup ? kDecodeCtas : 0;
+  const int blocks =
+      decode + (paged_single(a.t.max_rows, group)
+                    ? 0
+                    : kChunkCtas * (2 * kChunkRows / kCombineRows));
   return launch_kernel(dim == 64 ? paged_combine_kernel<T, 64>
                                  : paged_combine_kernel<T, 128>,
-                       dim3(a.t.rows), dim3(kCombineThreads), 0, stream, true,
-                       a);
+                       dim3(blocks), dim3(kCombineThreads), 0, stream, true, a,
+                       decode);
 }
 
 }  // namespace

@@ -86,7 +86,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int kvh = a.t.kv_heads, group = a.heads / kvh;
   const int QB = chunk_queries(group);
-  allow_dependents();
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.kv_full[i], 1);
@@ -104,17 +103,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == 9)
     tc::alloc(&s.tmem, kColumns);
-  bool broken;
-  const int64_t total =
-      paged_total(
-          a.t,
-          [&](const PagedSequence& q) {
-            return chunk_sequence_units(q, group, a.window);
-          },
-          broken) *
-      kvh;
-  if (broken && blockIdx.x == 0)
+  if (tid == 0) {
+    prefetch_map(&a.kmap);
+    prefetch_map(&a.vmap);
+  }
+  if (!a.behind_decode)
+    grid_dependency_wait();
+  allow_dependents();
+  const auto units = [&](const PagedSequence& q) {
+    return chunk_sequence_units(q, group, a.window);
+  };
+  const PagedLine line(a.t, units);
+  if (line.broken && blockIdx.x == 0 && warp == 0)
     report_error(kErrPagedTable);
+  const int64_t total = line.total * kvh;
   const int64_t share = paged_share(total, gridDim.x, kChunkMinUnits);
   const int64_t begin = share * blockIdx.x, end = min(begin + share, total);
   tc::fence_before();
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int per = 128 / a.box_rows;  // boxes of a slab
     uint32_t loads = 0;
     for (int64_t at = begin;
-         ok && chunk_segment(a.t, group, a.window, at, end, g); at += g.count)
+         ok && chunk_segment(line, group, a.window, at, end, g); at += g.count)
       for (int i = 0; i < 2 * g.count && ok; ++i, ++loads) {
         const int st = loads % kStages;
         if (loads >= kStages)
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- every MMA, one thread
     uint32_t loads = 0, tiles[2] = {0, 0}, segments[2] = {0, 0};
     for (int64_t at = begin;
-         ok && chunk_segment(a.t, group, a.window, at, end, g);
+         ok && chunk_segment(line, group, a.window, at, end, g);
          at += g.count, loads += 2 * g.count) {
       const int two = g.q.n - g.pair * 2 * QB > QB;  // row tile 1 is there
       if (lane == 0) {
@@ -261,8 +263,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, kErrPagedWait));
     };
     uint32_t loads = 0, tiles = 0, segments = 0;
+    PagedRecord record{0, 0, 0, 0, 0, 0};
     for (int64_t at = begin;
-         ok && chunk_segment(a.t, group, a.window, at, end, g);
+         ok && chunk_segment(line, group, a.window, at, end, g);
          at += g.count, loads += 2 * g.count) {
       const int q0 = g.pair * 2 * QB;
       const int qlast = min(g.q.n, q0 + 2 * QB) - 1;
@@ -503,10 +506,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                 reinterpret_cast<const uint4*>(y)[k];
         }
       }
+      if (!whole && g.u0 == 0)
+        record = paged_record(at, share, slot, g.n_units, g.q, g.pair, g.h);
       tiles += g.count;
       ++segments;
     }
+    if (tid == 0)
+      reinterpret_cast<PagedRecord*>(
+          a.chunk_part +
+          size_t(2 * kChunkCtas) * 256 * (DIM + 2))[blockIdx.x] = record;
+    // pairs of row tiles that see no key
+    for (int j = blockIdx.x; j < a.t.sequences; j += gridDim.x) {
+      const PagedSequence q = paged_sequence(a.t, j);
+      const int pairs = q.length < q.n ? chunk_pairs(q, group) : 0;
+      int lo;
+      for (int p = 0; p < pairs; ++p) {
+        if (chunk_units(q, group, a.window, p, lo))
+          continue;
+        for (int i = p * 2 * QB + warp; i < min(q.n, (p + 1) * 2 * QB);
+             i += 8) {
+          const size_t row = size_t(q.row0) + i;
+          for (int e = lane; e < a.heads * DIM; e += 32)
+            static_cast<T*>(a.out)[row * a.ldo + e] = from_float<T>(0);
+          for (int e = lane; a.lse && e < a.heads; e += 32)
+            a.lse[row * a.heads + e] = -INFINITY;
+        }
+      }
+    }
   }
+  if (a.behind_decode)
+    grid_dependency_wait();  // this grid ends after the decode kernel's
   tc::fence_before();
   __syncthreads();
   if (warp == 9) {
@@ -523,7 +552,7 @@ cudaError_t launch(const PagedAttentionArgs& a, cudaStream_t stream) {
           ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem))
     return e;
   return launch_kernel(kernel, dim3(kChunkCtas), dim3(kThreads), smem, stream,
-                       false, a);
+                       true, a);
 }
 template <typename T>
 cudaError_t launch(const PagedAttentionArgs& a, int dim, cudaStream_t stream) {
@@ -533,7 +562,8 @@ cudaError_t launch(const PagedAttentionArgs& a, int dim, cudaStream_t stream) {
 }  // namespace
 
 size_t paged_chunk_floats(int dim) {
-  return size_t(2 * kChunkCtas) * 256 * (dim + 2);
+  return size_t(2 * kChunkCtas) * 256 * (dim + 2) +
+         kChunkCtas * sizeof(PagedRecord) / 4;
 }
 
 cudaError_t launch_paged_chunk(const PagedAttentionArgs& a, uint32_t type,

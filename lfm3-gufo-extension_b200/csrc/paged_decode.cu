@@ -92,45 +92,60 @@ __global__ void __launch_bounds__(kThreads, 2)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int kvh = a.t.kv_heads, group = a.heads / kvh;
-  allow_dependents();
   if (lane == 0) {
     for (int i = 0; i < kStages; ++i)
       mbar_init(&s.full[warp][i], 1);
     fence_barrier_init();
+    prefetch_map(&a.kmap16);
+    prefetch_map(&a.vmap16);
   }
+  // what earlier kernels wrote is there; kernels launched behind this one may
+  // start once every block is past this point
+  grid_dependency_wait();
+  allow_dependents();
   const auto units = [&](const PagedSequence& q) {
     return int64_t(decode_units(q, group, a.window));
   };
-  bool broken;
-  const int64_t total = paged_total(a.t, units, broken) * kvh;
-  if (broken && blockIdx.x == 0)
+  const PagedLine line(a.t, units);
+  if (line.broken && blockIdx.x == 0 && warp == 0)
     report_error(kErrPagedTable);
+  const int64_t total = line.total * kvh;
   const int64_t share = paged_share(total, gridDim.x, kDecodeMinUnits);
-  int64_t at = share * blockIdx.x;
-  const int64_t end = min(at + share, total);
-  const bool starts_here = at < end;
-  int64_t index = -1, before = 0;  // the current sequence
-  int seq = 0;
-  PagedSequence q{};
+  const int64_t begin = share * blockIdx.x, end = min(begin + share, total);
+  PagedRecord record{0, 0, 0, 0, 0, 0};
   uint32_t used = 0;  // buffers this warp has filled so far
   const int fg = lane / 4, cq = lane % 4, mj = lane / 8, mrow = lane % 8;
   __syncwarp();
 
-  for (bool first_segment = true; starts_here && at < end;
-       first_segment = false) {
+  for (int64_t at = begin, next; at < end; at = next) {
     // ---- the segment: units [u0, u0 + count) of KV head h of sequence seq
-    if (index < 0 || at >= index) {
-      if (!paged_find(a.t, units, at / kvh, seq, q, before))
-        break;
-      int lo;
-      index = (before + paged_units(q, a.window, 0, 0, kDecodeKeys, lo)) * kvh;
-    }
-    int lo_unit;
+    int seq, lo_unit;
+    PagedSequence q{};
+    int64_t before;
+    if (!line.find(unit_div(at, kvh), seq, q, before))
+      break;
     const int n_units = paged_units(q, a.window, 0, 0, kDecodeKeys, lo_unit);
     const int64_t rel = at - before * kvh;
-    const int h = int(rel / n_units), u0 = int(rel % n_units);
+    const int h = int(unit_div(rel, n_units));
+    const int u0 = int(rel - int64_t(h) * n_units);
     const int count = int(min(int64_t(n_units - u0), end - at));
-    at += count;
+    next = at + count;
+    // ---- the group's queries are on their way while the page ids come
+    const int r = q.row0;
+    constexpr int kPerWarp = 8 * NT / kWarps;
+    float xq[kPerWarp][DIM / 32];
+#pragma unroll
+    for (int jj = 0; jj < kPerWarp; ++jj) {
+      const int j = warp + jj * kWarps;
+#pragma unroll
+      for (int i = 0; i < DIM / 32; ++i)
+        xq[jj][i] =
+            j < group
+                ? to_float(static_cast<const T*>(
+                      a.q)[size_t(r) * a.ldq + size_t(h * group + j) * DIM +
+                           lane + 32 * i])
+                : 0.0F;
+    }
     int first_key, last_key;
     paged_key_range(q, a.window, 0, 0, first_key, last_key);
     const int mine = (count - warp + kWarps - 1) / kWarps;  // this warp's
@@ -164,19 +179,15 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int i = 0; i < kStages; ++i)
       issue(i);
 
-    // ---- the group's queries, each scaled to fp16's range by a power of two
-    const int r = q.row0;
-    for (int j = warp; j < 8 * NT; j += kWarps) {
-      float x[DIM / 32];
+    // ---- the queries, each scaled to fp16's range by a power of two
+#pragma unroll
+    for (int jj = 0; jj < kPerWarp; ++jj) {
+      const int j = warp + jj * kWarps;
+      const float(&x)[DIM / 32] = xq[jj];
       float top = 0;
 #pragma unroll
-      for (int i = 0; i < DIM / 32; ++i) {
-        x[i] = j < group ? to_float(static_cast<const T*>(
-                               a.q)[size_t(r) * a.ldq +
-                                    size_t(h * group + j) * DIM + lane + 32 * i])
-                         : 0.0F;
+      for (int i = 0; i < DIM / 32; ++i)
         top = fmaxf(top, fabsf(x[i]));
-      }
       const float scale = row_scale(warp_max(top));
 #pragma unroll
       for (int i = 0; i < DIM / 32; ++i) {
@@ -325,7 +336,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int i = 0; i < kStages && i < mine; ++i)
         mbar_wait(&s.full[warp][(used + i) % kStages],
                   ((used + i) / kStages) & 1, kErrPagedWait);
-      return;
+      record.parts = 0;
+      break;
     }
     used += mine > 0 ? mine : 0;
 
@@ -371,7 +383,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncthreads();
     const bool whole = count == n_units;
-    const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
+    const int slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
+    if (!whole && u0 == 0)
+      record = paged_record(at, share, slot, n_units, q, 0, h);
     float* po = a.decode_part + size_t(slot) * group * DIM;
     float* pm = a.decode_part + size_t(2 * kDecodeCtas) * group * DIM +
                 size_t(slot) * group * 2;
@@ -400,6 +414,20 @@ __global__ void __launch_bounds__(kThreads, 2)
     fence_proxy_async();
     __syncthreads();
   }
+  // rows that see no key (idle sequences)
+  for (int j = blockIdx.x; j < a.t.sequences; j += gridDim.x) {
+    const PagedSequence q = paged_sequence(a.t, j);
+    if (paged_single(q.n, group) && decode_units(q, group, a.window) == 0) {
+      for (int i = tid; i < a.heads * DIM; i += kThreads)
+        static_cast<T*>(a.out)[size_t(q.row0) * a.ldo + i] = from_float<T>(0);
+      for (int i = tid; a.lse && i < a.heads; i += kThreads)
+        a.lse[size_t(q.row0) * a.heads + i] = -INFINITY;
+    }
+  }
+  if (tid == 0)
+    reinterpret_cast<PagedRecord*>(
+        a.decode_part +
+        size_t(2 * kDecodeCtas) * group * (DIM + 2))[blockIdx.x] = record;
 }
 
 template <typename T, int DIM, int NT>
@@ -411,7 +439,7 @@ cudaError_t launch(const PagedAttentionArgs& a, cudaStream_t stream) {
           ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem))
     return e;
   return launch_kernel(kernel, dim3(kDecodeCtas), dim3(kThreads), smem, stream,
-                       false, a);
+                       true, a);
 }
 template <typename T>
 cudaError_t launch(const PagedAttentionArgs& a, int dim, cudaStream_t stream) {
@@ -425,7 +453,8 @@ cudaError_t launch(const PagedAttentionArgs& a, int dim, cudaStream_t stream) {
 
 size_t paged_decode_floats(int dim, int group) {
   return group > kDecodeMaxGroup ? 0
-                                 : size_t(2 * kDecodeCtas) * group * (dim + 2);
+                                 : size_t(2 * kDecodeCtas) * group * (dim + 2) +
+                                       kDecodeCtas * sizeof(PagedRecord) / 4;
 }
 
 cudaError_t launch_paged_decode(const PagedAttentionArgs& a, uint32_t type,

@@ -8,9 +8,10 @@
 // (sequence, row tile, KV head) inside a block's range is a segment. A segment
 // that holds all the tiles writes the output; otherwise it leaves maxima, sums
 // and unnormalised outputs in a slot of the workspace (a block has at most two
-// such segments, its first and its last: slots 2 b and 2 b + 1), and the
-// combine kernel, which finds the same places by the same rules, merges them
-// in key order.
+// such segments, its first and its last: slots 2 b and 2 b + 1). The block
+// that holds a split stretch's first tiles (at most one such stretch begins in
+// a block) also leaves a record of it, and the combine kernel merges record by
+// record, in key order.
 #pragma once
 #include "paged.cuh"
 
@@ -94,57 +95,81 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
   return v;
 }
 
-// Sum of units(sequence) over the batch, and whether a sequence is broken
-// (warp-wide).
-template <typename Units>
-__device__ int64_t paged_total(const PagedTables& t, Units units,
-                               bool& broken) {
-  int64_t sum = 0;
-  broken = false;
-  for (int s = threadIdx.x % 32; s < t.sequences; s += 32) {
-    const PagedSequence q = paged_sequence(t, s);
-    broken |= q.broken;
-    sum += units(q);
-  }
-  return warp_sum64(sum);
+// Quotient of a unit number by a positive count (64-bit division is a long
+// sequence of instructions, and lines of 2^32 units are rare).
+__device__ __forceinline__ int64_t unit_div(int64_t a, int b) {
+  return uint64_t(a) >> 32 ? a / b : int64_t(uint32_t(a) / uint32_t(b));
 }
 
-// The sequence that holds unit `at` of the line of units(sequence), its
-// numbers, and the units before it (warp-wide). False past the end.
+// The line of units(sequence) of a batch (all members warp-wide). The first
+// 32 sequences' entries stay in registers, a lane each: for batches of up to
+// 32 the tables are read once.
 template <typename Units>
-__device__ bool paged_find(const PagedTables& t, Units units, int64_t at,
-                           int& s, PagedSequence& q, int64_t& before) {
-  const int lane = threadIdx.x % 32;
-  int64_t sum = 0;
-  for (int s0 = 0; s0 < t.sequences; s0 += 32) {
-    PagedSequence mine{0, 0, 0, true};
-    int64_t u = 0;
-    if (s0 + lane < t.sequences) {
-      mine = paged_sequence(t, s0 + lane);
-      u = units(mine);
+struct PagedLine {
+  const PagedTables& t;
+  Units units;
+  PagedSequence own;  // sequence `lane`
+  int64_t own_units;
+  int64_t total;  // units of the whole batch
+  bool broken;    // this lane met a broken sequence
+
+  __device__ PagedLine(const PagedTables& tables, Units u)
+      : t(tables), units(u), own{0, 0, 0, false}, own_units(0), total(0),
+        broken(false) {
+    const int lane = threadIdx.x % 32;
+    for (int s = lane; s < t.sequences; s += 32) {
+      const PagedSequence q = paged_sequence(t, s);
+      const int64_t n = units(q);
+      broken |= q.broken;
+      total += n;
+      if (s == lane) {
+        own = q;
+        own_units = n;
+      }
     }
-    int64_t inc = u;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o)
-        inc += x;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, sum + inc > at);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      s = s0 + l;
-      q.row0 = __shfl_sync(0xffffffffu, mine.row0, l);
-      q.n = __shfl_sync(0xffffffffu, mine.n, l);
-      q.length = __shfl_sync(0xffffffffu, mine.length, l);
-      q.broken = false;
-      before = sum + __shfl_sync(0xffffffffu, inc - u, l);
-      return true;
-    }
-    sum += __shfl_sync(0xffffffffu, inc, 31);
+    total = warp_sum64(total);
   }
-  return false;
-}
+
+  // The sequence that holds unit `at`, its numbers, and the units before it.
+  // False past the end.
+  __device__ bool find(int64_t at, int& s, PagedSequence& q,
+                       int64_t& before) const {
+    const int lane = threadIdx.x % 32;
+    int64_t sum = 0;
+    for (int s0 = 0; s0 < t.sequences; s0 += 32) {
+      PagedSequence mine = own;
+      int64_t u = own_units;
+      if (s0 > 0) {
+        mine = PagedSequence{0, 0, 0, false};
+        u = 0;
+        if (s0 + lane < t.sequences) {
+          mine = paged_sequence(t, s0 + lane);
+          u = units(mine);
+        }
+      }
+      int64_t inc = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o)
+          inc += x;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, sum + inc > at);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        s = s0 + l;
+        q.row0 = __shfl_sync(0xffffffffu, mine.row0, l);
+        q.n = __shfl_sync(0xffffffffu, mine.n, l);
+        q.length = __shfl_sync(0xffffffffu, mine.length, l);
+        q.broken = false;
+        before = sum + __shfl_sync(0xffffffffu, inc - u, l);
+        return true;
+      }
+      sum += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return false;
+  }
+};
 
 // One block's next piece of the chunks' line: units u0 .. u0 + count - 1 (of
 // n_units, the first of them key tile `lo_unit`) of a pair of row tiles and a
@@ -155,15 +180,12 @@ struct ChunkSegment {
   int n_units, lo_unit, u0, count;
 };
 // The segment at unit `at` of a range that ends at `end` (warp-wide).
-__device__ inline bool chunk_segment(const PagedTables& t, int group,
-                                     int window, int64_t at, int64_t end,
-                                     ChunkSegment& g) {
-  const int lane = threadIdx.x % 32, kvh = t.kv_heads;
-  const auto units = [&](const PagedSequence& q) {
-    return chunk_sequence_units(q, group, window);
-  };
+template <typename Line>
+__device__ bool chunk_segment(const Line& line, int group, int window,
+                              int64_t at, int64_t end, ChunkSegment& g) {
+  const int lane = threadIdx.x % 32, kvh = line.t.kv_heads;
   int64_t before;
-  if (at >= end || !paged_find(t, units, at / kvh, g.seq, g.q, before))
+  if (at >= end || !line.find(unit_div(at, kvh), g.seq, g.q, before))
     return false;
   const int pairs = chunk_pairs(g.q, group);
   int64_t rel = at - before * kvh;
@@ -186,8 +208,8 @@ __device__ inline bool chunk_segment(const PagedTables& t, int group,
       rel -= __shfl_sync(0xffffffffu, inc - mine, l);
       g.pair = p0 + l;
       g.n_units = chunk_units(g.q, group, window, g.pair, g.lo_unit);
-      g.h = int(rel / g.n_units);
-      g.u0 = int(rel % g.n_units);
+      g.h = int(unit_div(rel, g.n_units));
+      g.u0 = int(rel - int64_t(g.h) * g.n_units);
       g.count = int(min(int64_t(g.n_units - g.u0), end - at));
       return true;
     }
@@ -196,39 +218,32 @@ __device__ inline bool chunk_segment(const PagedTables& t, int group,
   return false;
 }
 
-// paged_find for the sequence that holds tensor row r.
-template <typename Units>
-__device__ bool paged_find_row(const PagedTables& t, Units units, int r,
-                               int& s, PagedSequence& q, int64_t& before) {
-  const int lane = threadIdx.x % 32;
-  int64_t sum = 0;
-  for (int s0 = 0; s0 < t.sequences; s0 += 32) {
-    PagedSequence mine{0, 0, 0, true};
-    if (s0 + lane < t.sequences)
-      mine = paged_sequence(t, s0 + lane);
-    const int64_t u = units(mine);
-    const unsigned hit = __ballot_sync(
-        0xffffffffu, mine.n > 0 && r >= mine.row0 && r < mine.row0 + mine.n);
-    if (!hit) {
-      sum += warp_sum64(u);
-      continue;
-    }
-    const int l = __ffs(hit) - 1;
-    s = s0 + l;
-    q.row0 = __shfl_sync(0xffffffffu, mine.row0, l);
-    q.n = __shfl_sync(0xffffffffu, mine.n, l);
-    q.length = __shfl_sync(0xffffffffu, mine.length, l);
-    q.broken = false;
-    before = sum + warp_sum64(lane < l ? u : 0);
-    return true;
-  }
-  return false;
-}
-
 // Units per block for a line of `total` units over `ctas` blocks.
 __device__ __forceinline__ int64_t paged_share(int64_t total, int ctas,
                                                int least) {
   return max((total + ctas - 1) / ctas, int64_t(least));
+}
+
+// A stretch that several blocks share: `parts` slots, the first `slot`, then
+// every second one from the next even number on (the blocks after the first
+// begin with it). parts 0: none begins in the block.
+struct PagedRecord {
+  int parts, slot;
+  int row0;  // tensor row of the sequence's first new row
+  int n;     // its new rows
+  int pair, h;
+};
+__device__ __forceinline__ int record_slot(const PagedRecord& r, int part) {
+  return part == 0 ? r.slot : (r.slot & ~1) + 2 * part;
+}
+// The record of a segment at unit `at` (units of its stretch: n_units) that
+// starts the stretch but does not end it.
+__device__ __forceinline__ PagedRecord paged_record(int64_t at, int64_t share,
+                                                    int slot, int n_units,
+                                                    const PagedSequence& q,
+                                                    int pair, int h) {
+  const int64_t past = at + n_units - 1 - int64_t(blockIdx.x) * share;
+  return {int(past / share) + 1, slot, q.row0, q.n, pair, h};
 }
 
 // ---- numbers of the softmax ---------------------------------------------------
