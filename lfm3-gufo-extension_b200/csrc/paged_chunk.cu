@@ -13,8 +13,8 @@
 // While the softmax of one row tile runs, the tensor cores work for the other:
 // the issue order is P_0 V, Q_0 K', P_1 V, Q_1 K', ... A row tile's next S
 // overwrites its P: tcgen05.mma of one thread run in order.
-// FP32 queries are two fp16 terms (two MMAs for S, both terms of P fill the
-// 128 columns of S, two MMAs for O): 22 bits where a 16-bit type has one term.
+// FP32 queries are two fp16 terms (two MMAs for S, two terms of P, which fill
+// the 128 columns of S, two MMAs for O): 22 bits where a 16-bit type has one.
 // Rows are scaled to fp16's range by a power of two first.
 // A row's probabilities are 2^(x - m) with a reference m that trails the
 // running maximum: 2^7 for the maximum when m moves, 2^15 at most before it
@@ -23,13 +23,17 @@
 // Masked keys. A key that a row does not see has probability 0, but 0 times a
 // NaN or an infinity in V would still reach the row's sums. In tiles where
 // some row sees less than all keys (the diagonal, a window's edge, the last
-// page's tail) the softmax warps therefore clear rows that no row of the pair
-// sees and values that are not finite before P V runs; rows that do see such a
-// value get it added at the end.
+// page's tail) a warp of its own therefore clears, between the copy and P V,
+// the rows that no row of the pair sees and the values that are not finite;
+// rows that do see such a value get it added at the end.
 // Blocks take equal shares of the batch's (row tile pair, KV head, key tile)
 // units (paged_plan.cuh), so one long history is split over all SMs. Warps:
-// 0-3 and 4-7 softmax and epilogue, 8 TMA, 9 tensor memory and (one thread)
-// every MMA. Every wait is bounded.
+// 0-3 and 4-7 softmax and epilogue (a warp loads, converts and writes its own
+// 32 rows, a row at a time over the lanes), 8 TMA, 9 tensor memory and (one
+// thread) every MMA, 10 the clearing, 11 works out the segments ahead of the
+// others. Every wait is bounded.
+#include <type_traits>
+
 #include "kernels.cuh"
 #include "paged.cuh"
 #include "paged_plan.cuh"
@@ -39,9 +43,10 @@
 namespace lfm3 {
 namespace {
 
-constexpr int kThreads = 10 * 32;
+constexpr int kThreads = 12 * 32;
 constexpr uint32_t kColS = 128, kColO = 256, kColumns = 512;
 constexpr uint32_t kSlab = 128 * 128;  // bytes of [128 rows][64 dims]
+constexpr int kPlanned = 4;            // segments worked out ahead
 // exponents (base 2) of a row's largest probability: when the reference
 // moves, and when it has to move again
 constexpr float kTopMoved = 7.0F, kTopLimit = 15.0F;
@@ -52,12 +57,15 @@ struct __align__(1024) ChunkSmem {
   static constexpr int kTile = kSlabs * kSlab;
   static constexpr int kStages =
       DIM == 128 ? (TERMS == 2 ? 3 : 5) : (TERMS == 2 ? 8 : 10);
-  uint8_t q[2][TERMS][kTile];
+  uint8_t q[2][TERMS][kTile];  // and the epilogue's rows
   uint8_t kv[kStages][kTile];  // K_0 V_0 K_1 V_1 ... in turn
-  uint64_t kv_full[kStages], kv_empty[kStages];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], idle;
+  // landed; landed and cleared; free again
+  uint64_t kv_full[kStages], kv_ready[kStages], kv_empty[kStages];
+  uint64_t q_full[2], q_free[2], s_full[2], p_full[2][3], o_full[2], idle;
+  uint64_t seg_full[kPlanned], seg_empty[kPlanned];
+  ChunkSegment seg[kPlanned];
   uint32_t tmem;
-  int odd_values;  // a value that is not finite was cleared in this segment
+  int odd_values;  // a value that is not finite was cleared
 };
 
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
@@ -71,6 +79,70 @@ __device__ __forceinline__ float2 bits_half2(uint32_t u) {
 __device__ __forceinline__ bool not_finite2(uint32_t u) {
   return (((u & 0x7C007C00u) + 0x04000400u) & 0x80008000u) != 0;
 }
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
+      "mov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\n"
+      "mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
+      "add.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+// 2^x on the FMA pipe: n = round(x), 2^(x - n) by a polynomial of degree 4
+// (least squares reweighted to equal relative error, 2.6e-6, two bits below
+// the half step of an fp16), n added to the exponent. Takes x up to 15 (NaN
+// and infinities make the row NaN before); below -125 it is 2^-125.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  x.x = fmaxf(x.x, -125.0F);
+  x.y = fmaxf(x.y, -125.0F);
+  const float2 magic = make_float2(12582912.0F, 12582912.0F);  // 1.5 * 2^23
+  const float2 back = make_float2(-12582912.0F, -12582912.0F);
+  const float2 t = add2(x, magic);
+  const float2 n = add2(t, back);
+  const float2 f = fma2(n, make_float2(-1.0F, -1.0F), x);
+  float2 p = make_float2(0x1.3997d4p-7F, 0x1.3997d4p-7F);
+  p = fma2(p, f, make_float2(0x1.ca1442p-5F, 0x1.ca1442p-5F));
+  p = fma2(p, f, make_float2(0x1.ec06dap-3F, 0x1.ec06dap-3F));
+  p = fma2(p, f, make_float2(0x1.62e0dcp-1F, 0x1.62e0dcp-1F));
+  p = fma2(p, f, make_float2(0x1.ffffe8p-1F, 0x1.ffffe8p-1F));
+  return make_float2(
+      __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
+// What a pair of row tiles sees: rows are the sequence's new rows q0 .. qlast.
+// Every row sees keys all_lo .. all_hi, some row any_lo .. any_hi.
+struct PairRange {
+  int q0, qlast, base, all_lo, all_hi, any_lo, any_hi;
+  __device__ PairRange(const ChunkSegment& g, int QB, int window) {
+    q0 = g.pair * 2 * QB;
+    qlast = min(g.q.n, q0 + 2 * QB) - 1;
+    base = g.q.length - g.q.n;
+    all_hi = base + q0;
+    any_hi = base + qlast;
+    all_lo = window > 0 ? max(0, base + qlast - window + 1) : 0;
+    any_lo = window > 0 ? max(0, base + q0 - window + 1) : 0;
+  }
+  // some row sees less than the whole tile
+  __device__ bool edge(int key0) const {
+    return key0 + kChunkKeys - 1 > all_hi || key0 < all_lo;
+  }
+};
 
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -89,53 +161,113 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.kv_full[i], 1);
+      mbar_init(&s.kv_ready[i], 1);
       mbar_init(&s.kv_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.q_full[i], 4);
+      mbar_init(&s.q_free[i], 4);
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.p_full[i], 4);
+      mbar_init(&s.p_full[i][0], 4);
+      mbar_init(&s.p_full[i][1], 4);
+      mbar_init(&s.p_full[i][2], 4);
       mbar_init(&s.o_full[i], 1);
+    }
+    for (int i = 0; i < kPlanned; ++i) {
+      mbar_init(&s.seg_full[i], 1);
+      mbar_init(&s.seg_empty[i], 11);  // every other warp
     }
     mbar_init(&s.idle, 1);
     s.odd_values = 0;
     fence_barrier_init();
-  }
-  if (warp == 9)
-    tc::alloc(&s.tmem, kColumns);
-  if (tid == 0) {
     prefetch_map(&a.kmap);
     prefetch_map(&a.vmap);
   }
+  if (warp == 9)
+    tc::alloc(&s.tmem, kColumns);
   if (!a.behind_decode)
     grid_dependency_wait();
   allow_dependents();
-  const auto units = [&](const PagedSequence& q) {
-    return chunk_sequence_units(q, group, a.window);
-  };
-  const PagedLine line(a.t, units);
-  if (line.broken && blockIdx.x == 0 && warp == 0)
-    report_error(kErrPagedTable);
-  const int64_t total = line.total * kvh;
-  const int64_t share = paged_share(total, gridDim.x, kChunkMinUnits);
-  const int64_t begin = share * blockIdx.x, end = min(begin + share, total);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = s.tmem;
   bool ok = true;
   ChunkSegment g;
-  // A barrier's phase is the parity of its completed uses: loads so far, and
-  // per row tile the key tiles and segments so far in which it took part.
+  uint32_t planned = 0;
+  // The next segment (warp-wide): false at the end of the block's share. A
+  // barrier's phase is the parity of its completed uses.
+  const auto next_segment = [&]() {
+    const uint32_t i = planned % kPlanned;
+    ok = ok && __all_sync(0xffffffffu,
+                          mbar_wait(&s.seg_full[i], (planned / kPlanned) & 1,
+                                    kErrPagedWait));
+    if (!ok)
+      return false;
+    g = s.seg[i];
+    __syncwarp();
+    if (lane == 0)
+      mbar_arrive(&s.seg_empty[i]);
+    ++planned;
+    return g.count > 0;
+  };
 
-  if (warp == 8) {
+  if (warp == 11) {
+    // ---- the block's segments, then one with count 0
+    const auto units = [&](const PagedSequence& q) {
+      return chunk_sequence_units(q, group, a.window);
+    };
+    const PagedLine line(a.t, units);
+    if (line.broken && blockIdx.x == 0)
+      report_error(kErrPagedTable);
+    const int64_t total = line.total * kvh;
+    const int64_t share = paged_share(total, kChunkCtas, kChunkMinUnits);
+    const int64_t begin = share * blockIdx.x, end = min(begin + share, total);
+    PagedRecord record{0, 0, 0, 0, 0, 0};
+    int64_t at = begin;
+    for (bool more = true; more && ok; ++planned) {
+      more = chunk_segment(line, group, a.window, at, end, g);
+      if (!more)
+        g.count = 0;
+      g.slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
+      if (more && g.count < g.n_units && g.u0 == 0)
+        record = paged_record(at, share, g.slot, g.n_units, g.q, g.pair, g.h);
+      at += g.count;
+      const uint32_t i = planned % kPlanned;
+      if (planned >= kPlanned)
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(&s.seg_empty[i],
+                                  ((planned / kPlanned) - 1) & 1,
+                                  kErrPagedWait));
+      if (lane == 0 && ok) {
+        s.seg[i] = g;
+        mbar_arrive(&s.seg_full[i]);
+      }
+      __syncwarp();
+    }
+    if (lane == 0)
+      reinterpret_cast<PagedRecord*>(
+          a.chunk_part +
+          size_t(2 * kChunkCtas) * 256 * (DIM + 2))[blockIdx.x] = record;
+  } else if (warp == 8) {
     // ---- TMA: K and V tiles, a lane per box
     const int per = 128 / a.box_rows;  // boxes of a slab
     uint32_t loads = 0;
-    for (int64_t at = begin;
-         ok && chunk_segment(line, group, a.window, at, end, g); at += g.count)
+    while (next_segment())
       for (int i = 0; i < 2 * g.count && ok; ++i, ++loads) {
         const int st = loads % kStages;
+        const int key0 = (g.lo_unit + g.u0 + i / 2) * kChunkKeys;
+        // boxes that hold rows of the sequence
+        const int boxes =
+            min(per, (g.q.length - key0 + a.box_rows - 1) / a.box_rows);
+        int row = 0;
+        if (lane < boxes * kSlabs)  // (at most 16 boxes of a key tile)
+          row = paged_row(a.t, a.t.table, g.seq,
+                          key0 + lane / kSlabs * a.box_rows);
+        if (row < 0) {
+          report_error(kErrPagedTable);
+          row = 0;
+        }
         if (loads >= kStages)
           ok = __all_sync(0xffffffffu,
                           mbar_wait(&s.kv_empty[st],
@@ -143,185 +275,280 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     kErrPagedWait));
         if (!ok)
           break;
-        const int key0 = (g.lo_unit + g.u0 + i / 2) * kChunkKeys;
-        // boxes that hold rows of the sequence
-        const int boxes =
-            min(per, (g.q.length - key0 + a.box_rows - 1) / a.box_rows);
         if (lane == 0)
           mbar_arrive_expect_tx(&s.kv_full[st],
                                 uint32_t(boxes * kSlabs * a.box_rows) * 128);
         __syncwarp();
-        for (int b = lane; b < boxes * kSlabs; b += 32) {
-          const int box = b / kSlabs, slab = b % kSlabs;
-          int row = paged_row(a.t, a.t.table, g.seq, key0 + box * a.box_rows);
-          if (row < 0) {
-            report_error(kErrPagedTable);
-            row = 0;
-          }
-          tma_load_3d(s.kv[st] + slab * kSlab + box * a.box_rows * 128,
-                      i % 2 ? &a.vmap : &a.kmap, 0, row, g.h * kSlabs + slab,
-                      &s.kv_full[st]);
-        }
+        if (lane < boxes * kSlabs)
+          tma_load_3d(s.kv[st] + lane % kSlabs * kSlab +
+                          lane / kSlabs * a.box_rows * 128,
+                      i % 2 ? &a.vmap : &a.kmap, 0, row,
+                      g.h * kSlabs + lane % kSlabs, &s.kv_full[st]);
       }
     // no copy may still be landing when the block exits
     for (uint32_t i = loads > kStages ? loads - kStages : 0; i < loads; ++i)
       mbar_wait(&s.kv_full[i % kStages], (i / kStages) & 1, kErrPagedWait);
-  } else if (warp == 9) {
-    // ---- every MMA, one thread
-    uint32_t loads = 0, tiles[2] = {0, 0}, segments[2] = {0, 0};
-    for (int64_t at = begin;
-         ok && chunk_segment(line, group, a.window, at, end, g);
-         at += g.count, loads += 2 * g.count) {
-      const int two = g.q.n - g.pair * 2 * QB > QB;  // row tile 1 is there
-      if (lane == 0) {
-        const auto full = [&](int i) {  // load i of this segment has landed
-          const uint32_t l = loads + i;
-          return mbar_wait(&s.kv_full[l % kStages], (l / kStages) & 1,
-                           kErrPagedWait);
-        };
-        const auto release = [&](int i) {
-          tc::commit(&s.kv_empty[(loads + i) % kStages]);
-        };
-        const auto scores = [&](int x, int j) {
-          const uint8_t* k = s.kv[(loads + 2 * j) % kStages];
+  } else if (warp == 10) {
+    // ---- clearing what masked rows must not meet in V
+    uint32_t loads = 0;
+    while (next_segment()) {
+      const PairRange range(g, QB, a.window);
+      for (int i = 0; i < 2 * g.count && ok; ++i, ++loads) {
+        const int st = loads % kStages;
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(&s.kv_full[st], (loads / kStages) & 1,
+                                  kErrPagedWait));
+        if (!ok)
+          break;
+        const int key0 = (g.lo_unit + g.u0 + i / 2) * kChunkKeys;
+        if (i % 2 && range.edge(key0)) {
+          uint8_t* v = s.kv[st];
+          bool odd = false;
+#pragma unroll 8
+          for (int e = lane; e < 128 * kSlabs * 8; e += 32) {
+            const int key = e / (8 * kSlabs), piece = e % (8 * kSlabs);
+            uint4* at16 = reinterpret_cast<uint4*>(
+                v + (piece / 8) * kSlab + tc::sw128_offset(key, piece % 8));
+            uint4 w = *at16;
+            const bool hidden =
+                key0 + key < range.any_lo || key0 + key > range.any_hi;
+            if (hidden) {
+              *at16 = make_uint4(0, 0, 0, 0);
+            } else if (not_finite2(w.x) || not_finite2(w.y) ||
+                       not_finite2(w.z) || not_finite2(w.w)) {
+              odd = true;
+              __half* h = reinterpret_cast<__half*>(&w);
 #pragma unroll
-          for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-            for (int k16 = 0; k16 < DIM / 16; ++k16)
-              tc::mma(tmem + x * kColS,
-                      tc::sw128_desc(s.q[x][t] + (k16 / 4) * kSlab) +
-                          (k16 % 4) * 2,
-                      tc::sw128_desc(k + (k16 / 4) * kSlab) + (k16 % 4) * 2,
-                      kIdescS, t > 0 || k16 > 0);
-          tc::commit(&s.s_full[x]);
-        };
-        const auto values = [&](int x, int j) {
-          const uint64_t v =
-              tc::sw128_mn_desc(s.kv[(loads + 2 * j + 1) % kStages], kSlab);
-#pragma unroll
-          for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-            for (int k16 = 0; k16 < 8; ++k16)
-              tc::mma_ts(tmem + kColO + x * 128,
-                         tmem + x * kColS + t * 64 + k16 * 8, v + k16 * 128,
-                         kIdescO, j > 0 || t > 0 || k16 > 0);
-        };
-        ok = mbar_wait(&s.q_full[0], segments[0] & 1, kErrPagedWait) && full(0);
-        if (ok) {
-          tc::fence_after();
-          scores(0, 0);
-          if (two) {
-            ok = mbar_wait(&s.q_full[1], segments[1] & 1, kErrPagedWait);
-            tc::fence_after();
-            if (ok)
-              scores(1, 0);
-          }
-          release(0);
-        }
-        for (int j = 0; j < g.count && ok; ++j) {
-          const bool more = j + 1 < g.count;
-          ok = full(2 * j + 1);
-          for (int x = 0; x < 1 + two && ok; ++x) {
-            ok = mbar_wait(&s.p_full[x], (tiles[x] + j) & 1, kErrPagedWait);
-            if (!ok)
-              break;
-            tc::fence_after();
-            values(x, j);
-            if (x == two)
-              release(2 * j + 1);
-            if (more) {
-              if (x == 0)
-                ok = full(2 * j + 2);
-              if (ok)
-                scores(x, j + 1);
-              if (x == two)
-                release(2 * j + 2);
-            } else {
-              tc::commit(&s.o_full[x]);
+              for (int k = 0; k < 8; ++k)
+                if ((__half_as_ushort(h[k]) & 0x7C00) == 0x7C00)
+                  h[k] = __ushort_as_half(0);
+              *at16 = w;
             }
           }
+          if (odd)
+            *reinterpret_cast<volatile int*>(&s.odd_values) = 1;
+          fence_proxy_async();
+          __syncwarp();
         }
-        for (int x = 0; x < 1 + two; ++x) {
-          tiles[x] += g.count;
-          ++segments[x];
+        if (lane == 0)
+          mbar_arrive(&s.kv_ready[st]);
+      }
+    }
+  } else if (warp == 9) {
+    // ---- every MMA, issued by one lane. The softmax warps leave this warp few
+    // issue slots, so what it needs is kept in uniform registers (a value of
+    // a warp-wide reduction is one) and worked out before each wait.
+    const bool lead = tc::elect();
+    const auto uniform = [](int v) {
+      return int(__reduce_max_sync(0xffffffffu, unsigned(v)));
+    };
+    const auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) ||
+             __all_sync(0xffffffffu, mbar_wait(bar, parity, kErrPagedWait));
+    };
+    const uint32_t tm = uniform(tmem);
+    const uint64_t qdesc = tc::sw128_desc(s.q[0][0]);
+    const uint64_t kdesc = tc::sw128_desc(s.kv[0]);
+    const uint64_t vdesc = tc::sw128_mn_desc(s.kv[0], kSlab);
+    constexpr uint32_t kStep = Smem::kTile / 16;  // a stage, a term
+    // stage and phase of the next load; uses of each row tile's barriers
+    uint32_t stage = 0, phase = 0, tiles0 = 0, tiles1 = 0;
+    uint32_t segment0 = 0, segment1 = 0;
+    const auto advance = [&]() {
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    };
+    const auto scores = [&](int x, uint32_t st) {
+      const uint64_t k = kdesc + st * kStep;
+      const uint64_t q = qdesc + x * TERMS * kStep;
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int k16 = 0; k16 < DIM / 16; ++k16) {
+          const int at = (k16 / 4) * (kSlab / 16) + (k16 % 4) * 2;
+          tc::mma_lead(tm + x * kColS, q + t * kStep + at, k + at, kIdescS,
+                       t > 0 || k16 > 0, lead);
+        }
+      tc::commit_lead(&s.s_full[x], lead);
+    };
+    // O += P V in the pieces the softmax hands over: keys 0 .. 63, 64 .. 95
+    // and 96 .. 127
+    const auto consume = [&](int x, uint32_t st, uint32_t more,
+                             uint32_t parity) {
+      const uint64_t v = vdesc + st * kStep;
+      const uint32_t p = tm + x * kColS, o = tm + kColO + x * 128;
+#pragma unroll
+      for (int third = 0; third < 3; ++third) {
+        if (!wait(&s.p_full[x][third], parity))
+          return false;
+        tc::fence_after();
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+          for (int k16 = third ? 2 + 2 * third : 0; k16 < 4 + 2 * third; ++k16)
+            tc::mma_ts_lead(o, p + k16 / 2 * 32 + t * 16 + k16 % 2 * 8,
+                            v + k16 * 128, kIdescO,
+                            t > 0 || k16 > 0 ? 1u : more, lead);
+      }
+      return true;
+    };
+    while (next_segment()) {
+      const int count = uniform(g.count);
+      // row tile 1 is there
+      const int two = uniform(g.q.n - g.pair * 2 * QB > QB);
+      ok = wait(&s.kv_ready[stage], phase) &&
+           wait(&s.q_full[0], segment0 & 1) &&
+           (!two || wait(&s.q_full[1], segment1 & 1));
+      if (!ok)
+        break;
+      tc::fence_after();
+      scores(0, stage);
+      if (two)
+        scores(1, stage);
+      tc::commit_lead(&s.kv_empty[stage], lead);
+      advance();
+      for (int j = 0; j < count; ++j) {
+        const uint32_t vs = stage, later = j > 0;
+        const bool more = j + 1 < count;
+        ok = wait(&s.kv_ready[vs], phase);
+        advance();
+        const uint32_t ks = stage;
+        if (more)
+          ok = ok && wait(&s.kv_ready[ks], phase);
+        ok = ok && consume(0, vs, later, (tiles0 + j) & 1);
+        if (!ok)
+          break;
+        if (!two)
+          tc::commit_lead(&s.kv_empty[vs], lead);
+        if (more)
+          scores(0, ks);
+        else
+          tc::commit_lead(&s.o_full[0], lead);
+        if (two) {
+          ok = consume(1, vs, later, (tiles1 + j) & 1);
+          if (!ok)
+            break;
+          tc::commit_lead(&s.kv_empty[vs], lead);
+          if (more)
+            scores(1, ks);
+          else
+            tc::commit_lead(&s.o_full[1], lead);
+        }
+        if (more) {
+          tc::commit_lead(&s.kv_empty[ks], lead);
+          advance();
         }
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok)
+        break;
+      tiles0 += count;
+      ++segment0;
+      if (two) {
+        tiles1 += count;
+        ++segment1;
+      }
     }
-    if (lane == 0) {
-      tc::commit(&s.idle);
-      mbar_wait(&s.idle, 0, kErrPagedWait);
-    }
+    tc::commit_lead(&s.idle, lead);
+    mbar_wait(&s.idle, 0, kErrPagedWait);
   } else {
     // ---- softmax and epilogue of row tile x: thread t owns row t
     const int x = warp / 4, t = tid % 128;
     const uint32_t lane_base = uint32_t((warp % 4) * 32) << 16;
     const uint32_t ts = tmem + lane_base + x * kColS;
     const uint32_t to = tmem + lane_base + kColO + x * 128;
+    // rows over the lanes: kRowLanes lanes of 16 bytes hold one row
+    constexpr int kVec = 16 / sizeof(T), kRowLanes = DIM / kVec;
+    constexpr int kRowsAtOnce = 32 / kRowLanes;
+    const int sub = lane / kRowLanes, part = lane % kRowLanes;
+    const int row_query = t / group, row_head = t % group;
     // a warp's lanes give up together: tensor-memory accesses are warp-wide
     const auto wait_all = [&](uint64_t* bar, uint32_t parity) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, kErrPagedWait));
     };
-    uint32_t loads = 0, tiles = 0, segments = 0;
-    PagedRecord record{0, 0, 0, 0, 0, 0};
-    for (int64_t at = begin;
-         ok && chunk_segment(line, group, a.window, at, end, g);
-         at += g.count, loads += 2 * g.count) {
-      const int q0 = g.pair * 2 * QB;
-      const int qlast = min(g.q.n, q0 + 2 * QB) - 1;
-      const int base = g.q.length - g.q.n;
-      if (x == 1 && g.q.n - q0 <= QB)
+    uint32_t tiles = 0, segments = 0;
+    while (next_segment()) {
+      const PairRange range(g, QB, a.window);
+      if (x == 1 && g.q.n - range.q0 <= QB)
         continue;
-      const int qi = q0 + x * QB + t / group, head = g.h * group + t % group;
-      const bool live = t < QB * group && qi < g.q.n;
+      const int qi = range.q0 + x * QB + row_query;
+      const int head = g.h * group + row_head;
+      const bool live = row_query < QB && qi < g.q.n;
       const size_t row = size_t(g.q.row0) + (live ? qi : 0);
-      // the row sees keys own - window + 1 .. own
-      const int own = live ? base + qi : -1;
+      // the row sees keys oldest .. own
+      const int own = live ? range.base + qi : -1;
       const int oldest = a.window > 0 ? max(0, own - a.window + 1) : 0;
-      // ... of which every row of the pair sees all_lo .. all_hi, some row
-      // any_lo .. any_hi
-      const int all_hi = base + q0, any_hi = base + qlast;
-      const int all_lo =
-          a.window > 0 ? max(0, base + qlast - a.window + 1) : 0;
-      const int any_lo = a.window > 0 ? max(0, base + q0 - a.window + 1) : 0;
-      float c;
+      float c = 0;
       {
-        // ---- Q row as fp16 terms
-        const T* src = static_cast<const T*>(a.q) + row * a.ldq +
-                       size_t(live ? head : 0) * DIM;
-        constexpr int kVec = 16 / sizeof(T);
-        uint4 raw[DIM / kVec];
-        float top = 0;
-#pragma unroll
-        for (int i = 0; i < DIM / kVec; ++i) {
-          raw[i] = live ? reinterpret_cast<const uint4*>(src)[i]
-                        : make_uint4(0, 0, 0, 0);
-          const T* e = reinterpret_cast<const T*>(&raw[i]);
-#pragma unroll
-          for (int k = 0; k < kVec; ++k)
-            top = fmaxf(top, fabsf(to_float(e[k])));
+        // ---- this warp's 32 rows of Q as fp16 terms
+        // (the row tile's warps have read their rows of the last segment)
+        if (segments > 0 &&
+            !wait_all(&s.q_free[x], (segments - 1) & 1)) {
+          ok = false;
+          break;
         }
-        const float scale = row_scale(top);
-        c = rsqrtf(float(DIM)) * kLog2e / scale;
+        const size_t offset = row * a.ldq + size_t(head) * DIM;
+        const unsigned alive = __ballot_sync(0xffffffffu, live);
+        constexpr int kBatch = 8;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 32; i0 += kBatch * kRowsAtOnce) {
+          uint4 raw[kBatch];
 #pragma unroll
-        for (int piece = 0; piece < DIM / 8; ++piece) {
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int e = piece * 8 + 2 * k;
-            const T* p = reinterpret_cast<const T*>(raw) + e;
-            const float v0 = to_float(p[0]) * scale, v1 = to_float(p[1]) * scale;
-            hi[k] = half2_bits(v0, v1);
-            const float2 back = bits_half2(hi[k]);
-            lo[k] = half2_bits(v0 - back.x, v1 - back.y);
+          for (int i = 0; i < kBatch; ++i) {
+            const int r = i0 + i * kRowsAtOnce + sub;
+            const size_t at =
+                __shfl_sync(0xffffffffu, (unsigned long long)offset, r & 31);
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (r < 32 && (alive >> r & 1))
+              raw[i] = *reinterpret_cast<const uint4*>(
+                  static_cast<const T*>(a.q) + at + part * kVec);
           }
-          const uint32_t off =
-              (piece / 8) * kSlab + tc::sw128_offset(t, piece % 8);
-          *reinterpret_cast<uint4*>(s.q[x][0] + off) =
-              make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if constexpr (TERMS == 2)
-            *reinterpret_cast<uint4*>(s.q[x][TERMS - 1] + off) =
-                make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int r = i0 + i * kRowsAtOnce + sub;
+            const T* e = reinterpret_cast<const T*>(&raw[i]);
+            float v[kVec], top = 0;
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) {
+              v[k] = to_float(e[k]);
+              top = fmaxf(top, fabsf(v[k]));
+            }
+#pragma unroll
+            for (int o = kRowLanes / 2; o; o >>= 1)
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float scale = row_scale(top);
+            // row r's owner is lane r
+            const float got = __shfl_sync(
+                0xffffffffu, scale,
+                (lane - i0 - i * kRowsAtOnce) * kRowLanes & 31);
+            if (lane - i0 - i * kRowsAtOnce >= 0 &&
+                lane - i0 - i * kRowsAtOnce < kRowsAtOnce)
+              c = rsqrtf(float(DIM)) * kLog2e / got;
+            uint32_t hi[kVec / 2], lo[kVec / 2];
+#pragma unroll
+            for (int k = 0; k < kVec / 2; ++k) {
+              const float v0 = v[2 * k] * scale, v1 = v[2 * k + 1] * scale;
+              hi[k] = half2_bits(v0, v1);
+              const float2 back = bits_half2(hi[k]);
+              lo[k] = half2_bits(v0 - back.x, v1 - back.y);
+            }
+            if (r < 32) {
+              const int piece = part * kVec / 8;
+              const uint32_t off =
+                  (piece / 8) * kSlab +
+                  tc::sw128_offset((warp % 4) * 32 + r, piece % 8);
+              if constexpr (TERMS == 2) {
+                *reinterpret_cast<uint2*>(s.q[x][0] + off + (part & 1) * 8) =
+                    make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(s.q[x][1] + off + (part & 1) * 8) =
+                    make_uint2(lo[0], lo[1]);
+              } else {
+                *reinterpret_cast<uint4*>(s.q[x][0] + off) =
+                    make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              }
+            }
+          }
         }
         fence_proxy_async();
         tc::fence_before();
@@ -329,7 +556,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0)
           mbar_arrive(&s.q_full[x]);
       }
-      float m = -INFINITY, l = 0;
+      float m = -INFINITY;
+      float2 sum0 = make_float2(0, 0), sum1 = sum0;
       for (int j = 0; j < g.count; ++j) {
         const int key0 = (g.lo_unit + g.u0 + j) * kChunkKeys;
         if (!wait_all(&s.s_full[x], (tiles + j) & 1)) {
@@ -337,108 +565,135 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc::fence_after();
-        uint32_t sv[128];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          tc::ld32(ts + i * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32 * i));
-        tc::wait_ld();
-        const bool edge = key0 + kChunkKeys - 1 > all_hi || key0 < all_lo;
-        if (edge) {
+        // half of S is read again for its probabilities: with all 128 values
+        // and the packed P live, registers would spill
+        const auto softmax = [&](auto edge_tile) {
+          constexpr bool EDGE = decltype(edge_tile)::value;
+          uint32_t v0[32], v1[32];
+          tc::ld32(ts + 64, v0);
+          tc::ld32(ts + 96, v1);
+          tc::wait_ld();
           const int hi = own - key0, lo = oldest - key0;
+          const auto mask = [&](uint32_t(&v)[32], int first) {
+            if constexpr (EDGE)
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i > hi || i < lo)
-              sv[i] = __float_as_uint(-INFINITY);
-          // clear what masked rows must not meet in V
-          const uint32_t ld = loads + 2 * j + 1;
-          if (!wait_all(&s.kv_full[ld % kStages], (ld / kStages) & 1)) {
-            ok = false;
-            break;
-          }
-          uint8_t* v = s.kv[ld % kStages];
-          for (int i = t; i < 128 * kSlabs * 8; i += 128) {
-            const int key = i / (8 * kSlabs), piece = i % (8 * kSlabs);
-            uint4* at16 = reinterpret_cast<uint4*>(
-                v + (piece / 8) * kSlab + tc::sw128_offset(key, piece % 8));
-            if (key0 + key < any_lo || key0 + key > any_hi) {
-              *at16 = make_uint4(0, 0, 0, 0);
-              continue;
+              for (int i = 0; i < 32; ++i)
+                if (first + i > hi || first + i < lo)
+                  v[i] = __float_as_uint(-INFINITY);
+          };
+          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          const auto largest = [&](const uint32_t(&v)[32]) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                tops[k] = max_nan(tops[k],
+                                  max_nan(__uint_as_float(v[i + k]),
+                                          __uint_as_float(v[i + k + 4])));
+          };
+          mask(v0, 64);
+          mask(v1, 96);
+          largest(v0);
+          largest(v1);
+          tc::ld32(ts, v0);
+          tc::ld32(ts + 32, v1);
+          tc::wait_ld();
+          mask(v0, 0);
+          mask(v1, 32);
+          largest(v0);
+          largest(v1);
+          const float top =
+              max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3])) * c;
+          const bool move = !(top <= m + kTopLimit);
+          if (__any_sync(0xffffffffu, move)) {
+            float alpha = 1;
+            if (move) {
+              alpha = ex2(m - (top - kTopMoved));
+              // a NaN or an infinite score makes the row NaN
+              m = top < INFINITY ? top - kTopMoved : NAN;
+              sum0 = make_float2(sum0.x * alpha, sum0.y * alpha);
+              sum1 = make_float2(sum1.x * alpha, sum1.y * alpha);
             }
-            uint4 w = *at16;
-            if (not_finite2(w.x) || not_finite2(w.y) || not_finite2(w.z) ||
-                not_finite2(w.w)) {
-              __half* e = reinterpret_cast<__half*>(&w);
+            // O follows the reference (P_{j-1} V_{j-1} was issued before S_j,
+            // which has completed)
+            if (j > 0) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if ((__half_as_ushort(e[k]) & 0x7C00) == 0x7C00)
-                  e[k] = __ushort_as_half(0);
-              // (the flag first: the other row tile may find zeros here)
-              *reinterpret_cast<volatile int*>(&s.odd_values) = 1;
-              __threadfence_block();
-              *at16 = w;
+              for (int i = 0; i < DIM / 32; ++i) {
+                uint32_t ov[32];
+                tc::ld32(to + i * 32, ov);
+                tc::wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  ov[k] = __float_as_uint(__uint_as_float(ov[k]) * alpha);
+                tc::st32(to + i * 32, ov);
+              }
             }
           }
-          fence_proxy_async();
-        }
-        float tops[4];
+          const float shift = m == -INFINITY ? 0.0F : -m;
+          const float2 c2 = make_float2(c, c);
+          const float2 shift2 = make_float2(shift, shift);
+          uint32_t ph[16], pl[16];
+          const auto compute = [&](const uint32_t(&v)[32]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          tops[i] = __uint_as_float(sv[i]);
-#pragma unroll
-        for (int i = 4; i < 128; ++i)
-          tops[i % 4] = fmaxf(tops[i % 4], __uint_as_float(sv[i]));
-        const float top =
-            fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * c;
-        const bool move = top > m + kTopLimit;
-        float alpha = 1;
-        if (move) {
-          alpha = ex2(m - (top - kTopMoved));
-          m = top - kTopMoved;
-          l *= alpha;
-        }
-        const float shift = m == -INFINITY ? 0.0F : -m;
-        uint32_t ph[64], pl[TERMS == 2 ? 64 : 1];
-        float sums[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          const float p0 = ex2(fmaf(__uint_as_float(sv[2 * i]), c, shift));
-          const float p1 = ex2(fmaf(__uint_as_float(sv[2 * i + 1]), c, shift));
-          sums[(2 * i) % 4] += p0;
-          sums[(2 * i + 1) % 4] += p1;
-          ph[i] = half2_bits(p0, p1);
-          if constexpr (TERMS == 2) {
-            const float2 back = bits_half2(ph[i]);
-            pl[i] = half2_bits(p0 - back.x, p1 - back.y);
-          }
-        }
-        l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          tc::st32(ts + i * 32,
-                   *reinterpret_cast<uint32_t(*)[32]>(ph + 32 * i));
-          if constexpr (TERMS == 2)
-            tc::st32(ts + 64 + i * 32,
-                     *reinterpret_cast<uint32_t(*)[32]>(pl + 32 * i));
-        }
-        // O follows the reference (P_{j-1} V_{j-1} was issued before S_j,
-        // which has completed)
-        if (j > 0 && __any_sync(0xffffffffu, move)) {
-#pragma unroll
-          for (int i = 0; i < DIM / 32; ++i) {
-            uint32_t ov[32];
-            tc::ld32(to + i * 32, ov);
-            tc::wait_ld();
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              ov[k] = __float_as_uint(__uint_as_float(ov[k]) * alpha);
-            tc::st32(to + i * 32, ov);
-          }
-        }
-        tc::wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(&s.p_full[x]);
+            for (int i = 0; i < 16; ++i) {
+              float2 p = fma2(make_float2(__uint_as_float(v[2 * i]),
+                                          __uint_as_float(v[2 * i + 1])),
+                              c2, shift2);
+              if (!EDGE && TERMS == 1 && i % 4 == 3) {
+                p = ex2_poly(p);
+              } else {
+                p.x = ex2(p.x);
+                p.y = ex2(p.y);
+              }
+              if (i % 2)
+                sum1 = add2(sum1, p);
+              else
+                sum0 = add2(sum0, p);
+              ph[i] = half2_bits(p.x, p.y);
+              if constexpr (TERMS == 2) {
+                const float2 back = bits_half2(ph[i]);
+                pl[i] = half2_bits(p.x - back.x, p.y - back.y);
+              } else {
+                (void)pl;
+              }
+            }
+          };
+          // P over S: the fp16 terms of keys 32 i .. + 31 take the 32 columns
+          // (16 a term) their scores were read from
+          const auto store = [&](int first) {
+            tc::st16(ts + first, ph);
+            if constexpr (TERMS == 2)
+              tc::st16(ts + first + 16, pl);
+          };
+          const auto arrive = [&](int third) {
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0)
+              mbar_arrive(&s.p_full[x][third]);
+          };
+          compute(v0);
+          store(0);
+          tc::ld32(ts + 64, v0);
+          compute(v1);
+          store(32);
+          tc::wait_ld();
+          mask(v0, 64);
+          tc::ld32(ts + 96, v1);
+          compute(v0);
+          arrive(0);
+          store(64);
+          tc::wait_ld();
+          mask(v1, 96);
+          compute(v1);
+          arrive(1);
+          store(96);
+          arrive(2);
+        };
+        if (range.edge(key0))
+          softmax(std::true_type{});
+        else
+          softmax(std::false_type{});
       }
       // ---- epilogue
       if (ok)
@@ -446,14 +701,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok)
         break;
       tc::fence_after();
+      const float l = (sum0.x + sum1.x) + (sum0.y + sum1.y);
       // (every tile's clearing precedes its P V, which precedes o_full)
       const bool odd = *reinterpret_cast<volatile int*>(&s.odd_values) != 0;
       const bool whole = g.count == g.n_units;
-      const int slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
-      float* po = a.chunk_part + size_t(slot) * 256 * DIM + (x * 128 + t) * 4;
+      float* po = a.chunk_part + size_t(g.slot) * 256 * DIM + (x * 128 + t) * 4;
       float factor = 1;
       if (whole) {
-        factor = l > 0 ? 1.0F / l : l == 0 ? 0.0F : l;
+        factor = l == 0 ? 0.0F : 1.0F / l;
         if (a.gate && live)
           factor /= 1 + expf(-to_float(static_cast<const T*>(
                             a.gate)[row * a.ldg + head]));
@@ -462,9 +717,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         float2* pm = reinterpret_cast<float2*>(
             a.chunk_part + size_t(2 * kChunkCtas) * 256 * DIM);
-        pm[slot * 256 + x * 128 + t] = make_float2(m, l);
+        pm[g.slot * 256 + x * 128 + t] = make_float2(m, l);
       }
-      T* out = static_cast<T*>(a.out) + row * a.ldo + size_t(head) * DIM;
+      // whole rows go through the warp's part of the Q buffer (16-byte piece
+      // i of row r at i ^ (r & 7)), then out a row at a time
+      uint8_t* stage = s.q[x][0] + (warp % 4) * 32 * DIM * sizeof(T);
+      constexpr int kPieces = DIM * sizeof(T) / 16;
 #pragma unroll
       for (int i = 0; i < DIM / 32; ++i) {
         uint32_t ov[32];
@@ -475,8 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int key = max(oldest, (g.lo_unit + g.u0) * kChunkKeys);
                key <= min(own, (g.lo_unit + g.u0 + g.count) * kChunkKeys - 1);
                ++key) {
-            const int k0 = key / kChunkKeys * kChunkKeys;
-            if (!(k0 + kChunkKeys - 1 > all_hi || k0 < all_lo))
+            if (!range.edge(key / kChunkKeys * kChunkKeys))
               continue;  // not a tile that was cleared
             const int pool = paged_row(a.t, a.t.table, g.seq, key);
             if (pool < 0)
@@ -495,26 +752,42 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<uint4*>(po + size_t(i * 8 + k) * 1024) =
                 make_uint4(ov[4 * k], ov[4 * k + 1], ov[4 * k + 2],
                            ov[4 * k + 3]);
-        } else if (live) {
-          alignas(16) T y[32];
+        } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            y[k] = from_float<T>(__uint_as_float(ov[k]) * factor);
+          for (int k = 0; k < 32 / kVec; ++k) {
+            alignas(16) T y[kVec];
 #pragma unroll
-          for (int k = 0; k < 32 * int(sizeof(T)) / 16; ++k)
-            reinterpret_cast<uint4*>(out + i * 32)[k] =
-                reinterpret_cast<const uint4*>(y)[k];
+            for (int e = 0; e < kVec; ++e)
+              y[e] = from_float<T>(__uint_as_float(ov[k * kVec + e]) * factor);
+            const int piece = i * (32 / kVec) + k;
+            *reinterpret_cast<uint4*>(
+                stage + (lane * kPieces + (piece ^ (lane & 7))) * 16) =
+                *reinterpret_cast<const uint4*>(y);
+          }
         }
       }
-      if (!whole && g.u0 == 0)
-        record = paged_record(at, share, slot, g.n_units, g.q, g.pair, g.h);
+      if (whole) {
+        __syncwarp();
+        const size_t offset = row * a.ldo + size_t(head) * DIM;
+        const unsigned alive = __ballot_sync(0xffffffffu, live);
+#pragma unroll 4
+        for (int i = 0; i < 32; i += kRowsAtOnce) {
+          const int r = i + sub;
+          const size_t at =
+              __shfl_sync(0xffffffffu, (unsigned long long)offset, r);
+          if (alive >> r & 1)
+            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at +
+                                      part * kVec) =
+                *reinterpret_cast<const uint4*>(
+                    stage + (r * kPieces + (part ^ (r & 7))) * 16);
+        }
+      }
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&s.q_free[x]);
       tiles += g.count;
       ++segments;
     }
-    if (tid == 0)
-      reinterpret_cast<PagedRecord*>(
-          a.chunk_part +
-          size_t(2 * kChunkCtas) * 256 * (DIM + 2))[blockIdx.x] = record;
     // pairs of row tiles that see no key
     for (int j = blockIdx.x; j < a.t.sequences; j += gridDim.x) {
       const PagedSequence q = paged_sequence(a.t, j);

@@ -173,11 +173,12 @@ struct PagedLine {
 
 // One block's next piece of the chunks' line: units u0 .. u0 + count - 1 (of
 // n_units, the first of them key tile `lo_unit`) of a pair of row tiles and a
-// KV head.
+// KV head, and the block's slot for it.
 struct ChunkSegment {
   PagedSequence q;
   int seq, pair, h;
   int n_units, lo_unit, u0, count;
+  int slot;
 };
 // The segment at unit `at` of a range that ends at `end` (warp-wide).
 template <typename Line>

@@ -89,16 +89,47 @@ __device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t a, uint64_t b,
       : "memory");
 }
 
+// True in one lane of a converged warp. A warp whose lanes all run the issuing
+// code, with only the instructions below under this predicate, keeps
+// descriptors in uniform registers; inside a branch of one thread each operand
+// would be moved there for every instruction.
+__device__ __forceinline__ bool elect() {
+  uint32_t e;
+  asm volatile(
+      "{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\n"
+      "selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(e));
+  return e != 0;
+}
+// D = A B^T (+ D), issued by the lane with `lead`.
+__device__ __forceinline__ void mma_lead(uint32_t d_tmem, uint64_t a,
+                                         uint64_t b, uint32_t idesc,
+                                         uint32_t accumulate, bool lead) {
+  asm volatile(
+      "{\n.reg .pred p, e;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 e, %5, 0;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
+          d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(uint32_t(lead))
+      : "memory");
+}
 // The same with A in tensor memory: lane = row, each 32-bit column two
 // consecutive K elements (adding 8 advances K by 16).
-__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem,
-                                       uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts_lead(uint32_t d_tmem, uint32_t a_tmem,
+                                            uint64_t b, uint32_t idesc,
+                                            uint32_t accumulate, bool lead) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
-          d_tmem),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n.reg .pred p, e;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 e, %5, 0;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::
+          "r"(d_tmem),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate), "r"(uint32_t(lead))
+      : "memory");
+}
+__device__ __forceinline__ void commit_lead(uint64_t* bar, bool lead) {
+  asm volatile(
+      "{\n.reg .pred e;\nsetp.ne.b32 e, %1, 0;\n"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 "
+      "[%0];\n}\n" ::"r"(smem_addr(bar)),
+      "r"(uint32_t(lead))
       : "memory");
 }
 
@@ -139,6 +170,15 @@ __device__ __forceinline__ void st32(uint32_t taddr, const uint32_t (&v)[32]) {
       "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
       "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
       "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+      "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+      "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void wait_ld() {
