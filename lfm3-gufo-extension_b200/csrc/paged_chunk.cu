@@ -32,8 +32,6 @@
 // 32 rows, a row at a time over the lanes), 8 TMA, 9 tensor memory and (one
 // thread) every MMA, 10 the clearing, 11 works out the segments ahead of the
 // others. Every wait is bounded.
-#include <type_traits>
-
 #include "kernels.cuh"
 #include "paged.cuh"
 #include "paged_plan.cuh"
@@ -230,9 +228,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!more)
         g.count = 0;
       g.slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
-      if (more && g.count < g.n_units && g.u0 == 0)
-        record = paged_record(at, share, g.slot, g.n_units, g.q, g.pair, g.h);
-      at += g.count;
       const uint32_t i = planned % kPlanned;
       if (planned >= kPlanned)
         ok = __all_sync(0xffffffffu,
@@ -244,6 +239,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&s.seg_full[i]);
       }
       __syncwarp();
+      if (more && g.count < g.n_units && g.u0 == 0)
+        record = paged_record(at, share, g.slot, g.n_units, g.q, g.pair, g.h);
+      at += g.count;
     }
     if (lane == 0)
       reinterpret_cast<PagedRecord*>(
@@ -253,38 +251,49 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- TMA: K and V tiles, a lane per box
     const int per = 128 / a.box_rows;  // boxes of a slab
     uint32_t loads = 0;
-    while (next_segment())
-      for (int i = 0; i < 2 * g.count && ok; ++i, ++loads) {
-        const int st = loads % kStages;
-        const int key0 = (g.lo_unit + g.u0 + i / 2) * kChunkKeys;
-        // boxes that hold rows of the sequence
+    while (next_segment()) {
+      // page ids are read a key tile ahead of their copies
+      const auto pool_row = [&](int j) {
+        const int key0 = (g.lo_unit + g.u0 + j) * kChunkKeys;
+        const int key = key0 + lane / kSlabs * a.box_rows;
+        // (at most 16 boxes of a key tile, each with rows of the sequence)
+        return j < g.count && lane < per * kSlabs && key < g.q.length
+                   ? paged_row(a.t, a.t.table, g.seq, key)
+                   : 0;
+      };
+      int next = pool_row(0);
+      for (int j = 0; j < g.count && ok; ++j) {
+        const int key0 = (g.lo_unit + g.u0 + j) * kChunkKeys;
         const int boxes =
             min(per, (g.q.length - key0 + a.box_rows - 1) / a.box_rows);
-        int row = 0;
-        if (lane < boxes * kSlabs)  // (at most 16 boxes of a key tile)
-          row = paged_row(a.t, a.t.table, g.seq,
-                          key0 + lane / kSlabs * a.box_rows);
+        int row = next;
+        next = pool_row(j + 1);
         if (row < 0) {
           report_error(kErrPagedTable);
           row = 0;
         }
-        if (loads >= kStages)
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait(&s.kv_empty[st],
-                                    ((loads / kStages) - 1) & 1,
-                                    kErrPagedWait));
-        if (!ok)
-          break;
-        if (lane == 0)
-          mbar_arrive_expect_tx(&s.kv_full[st],
-                                uint32_t(boxes * kSlabs * a.box_rows) * 128);
-        __syncwarp();
-        if (lane < boxes * kSlabs)
-          tma_load_3d(s.kv[st] + lane % kSlabs * kSlab +
-                          lane / kSlabs * a.box_rows * 128,
-                      i % 2 ? &a.vmap : &a.kmap, 0, row,
-                      g.h * kSlabs + lane % kSlabs, &s.kv_full[st]);
+#pragma unroll
+        for (int v = 0; v < 2; ++v, ++loads) {
+          const int st = loads % kStages;
+          if (loads >= kStages)
+            ok = ok && __all_sync(0xffffffffu,
+                                  mbar_wait(&s.kv_empty[st],
+                                            ((loads / kStages) - 1) & 1,
+                                            kErrPagedWait));
+          if (!ok)
+            break;
+          if (lane == 0)
+            mbar_arrive_expect_tx(&s.kv_full[st],
+                                  uint32_t(boxes * kSlabs * a.box_rows) * 128);
+          __syncwarp();
+          if (lane < boxes * kSlabs)
+            tma_load_3d(s.kv[st] + lane % kSlabs * kSlab +
+                            lane / kSlabs * a.box_rows * 128,
+                        v ? &a.vmap : &a.kmap, 0, row,
+                        g.h * kSlabs + lane % kSlabs, &s.kv_full[st]);
+        }
       }
+    }
     // no copy may still be landing when the block exits
     for (uint32_t i = loads > kStages ? loads - kStages : 0; i < loads; ++i)
       mbar_wait(&s.kv_full[i % kStages], (i / kStages) & 1, kErrPagedWait);
@@ -490,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const size_t offset = row * a.ldq + size_t(head) * DIM;
         const unsigned alive = __ballot_sync(0xffffffffu, live);
-        constexpr int kBatch = 8;
+        constexpr int kBatch = kRowsAtOnce > 2 ? 32 / kRowsAtOnce : 16;
 #pragma unroll 1
         for (int i0 = 0; i0 < 32; i0 += kBatch * kRowsAtOnce) {
           uint4 raw[kBatch];
@@ -524,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 (lane - i0 - i * kRowsAtOnce) * kRowLanes & 31);
             if (lane - i0 - i * kRowsAtOnce >= 0 &&
                 lane - i0 - i * kRowsAtOnce < kRowsAtOnce)
-              c = rsqrtf(float(DIM)) * kLog2e / got;
+              c = got;
             uint32_t hi[kVec / 2], lo[kVec / 2];
 #pragma unroll
             for (int k = 0; k < kVec / 2; ++k) {
@@ -550,6 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+        c = rsqrtf(float(DIM)) * kLog2e / c;
         fence_proxy_async();
         tc::fence_before();
         __syncwarp();
@@ -565,135 +575,139 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc::fence_after();
-        // half of S is read again for its probabilities: with all 128 values
-        // and the packed P live, registers would spill
-        const auto softmax = [&](auto edge_tile) {
-          constexpr bool EDGE = decltype(edge_tile)::value;
-          uint32_t v0[32], v1[32];
-          tc::ld32(ts + 64, v0);
-          tc::ld32(ts + 96, v1);
+        // S is read twice, for the maximum and for the probabilities: with
+        // all 128 values and the packed P live, registers would spill
+        const bool edge = range.edge(key0);
+        const int hi = own - key0, lo = oldest - key0;
+        // columns first .. first + 31 that the row does not see become -inf
+        const auto mask = [&](uint32_t(&v)[32], int first) {
+          if (!edge)
+            return;
+          const int a0 = max(lo - first, 0), a1 = min(hi - first, 31);
+          const uint32_t seen =
+              a1 < a0 || a0 > 31 ? 0u
+                                 : (0xffffffffu >> (31 - (a1 - a0))) << a0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(seen >> i & 1))
+              v[i] = __float_as_uint(-INFINITY);
+        };
+        uint32_t v0[32], v1[32];
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const auto largest = [&](const uint32_t(&v)[32]) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tops[k] = max_nan(tops[k],
+                                max_nan(__uint_as_float(v[i + k]),
+                                        __uint_as_float(v[i + k + 4])));
+        };
+#pragma unroll 1
+        for (int first = 64; first >= 0; first -= 64) {
+          tc::ld32(ts + first, v0);
+          tc::ld32(ts + first + 32, v1);
           tc::wait_ld();
-          const int hi = own - key0, lo = oldest - key0;
-          const auto mask = [&](uint32_t(&v)[32], int first) {
-            if constexpr (EDGE)
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (first + i > hi || first + i < lo)
-                  v[i] = __float_as_uint(-INFINITY);
-          };
-          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          const auto largest = [&](const uint32_t(&v)[32]) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 8)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                tops[k] = max_nan(tops[k],
-                                  max_nan(__uint_as_float(v[i + k]),
-                                          __uint_as_float(v[i + k + 4])));
-          };
-          mask(v0, 64);
-          mask(v1, 96);
+          mask(v0, first);
+          mask(v1, first + 32);
           largest(v0);
           largest(v1);
-          tc::ld32(ts, v0);
-          tc::ld32(ts + 32, v1);
-          tc::wait_ld();
-          mask(v0, 0);
-          mask(v1, 32);
-          largest(v0);
-          largest(v1);
-          const float top =
-              max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3])) * c;
-          const bool move = !(top <= m + kTopLimit);
-          if (__any_sync(0xffffffffu, move)) {
-            float alpha = 1;
-            if (move) {
-              alpha = ex2(m - (top - kTopMoved));
-              // a NaN or an infinite score makes the row NaN
-              m = top < INFINITY ? top - kTopMoved : NAN;
-              sum0 = make_float2(sum0.x * alpha, sum0.y * alpha);
-              sum1 = make_float2(sum1.x * alpha, sum1.y * alpha);
-            }
-            // O follows the reference (P_{j-1} V_{j-1} was issued before S_j,
-            // which has completed)
-            if (j > 0) {
+        }
+        const float top =
+            max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3])) * c;
+        const bool move = !(top <= m + kTopLimit);
+        if (__any_sync(0xffffffffu, move)) {
+          float alpha = 1;
+          if (move) {
+            alpha = ex2(m - (top - kTopMoved));
+            // a NaN or an infinite score makes the row NaN
+            m = top < INFINITY ? top - kTopMoved : NAN;
+            sum0 = make_float2(sum0.x * alpha, sum0.y * alpha);
+            sum1 = make_float2(sum1.x * alpha, sum1.y * alpha);
+          }
+          // O follows the reference (P_{j-1} V_{j-1} was issued before S_j,
+          // which has completed)
+          if (j > 0) {
+#pragma unroll 1
+            for (int i = 0; i < DIM / 16; ++i) {
+              uint32_t ov[16];
+              tc::ld16(to + i * 16, ov);
+              tc::wait_ld();
 #pragma unroll
-              for (int i = 0; i < DIM / 32; ++i) {
-                uint32_t ov[32];
-                tc::ld32(to + i * 32, ov);
-                tc::wait_ld();
-#pragma unroll
-                for (int k = 0; k < 32; ++k)
-                  ov[k] = __float_as_uint(__uint_as_float(ov[k]) * alpha);
-                tc::st32(to + i * 32, ov);
-              }
+              for (int k = 0; k < 16; ++k)
+                ov[k] = __float_as_uint(__uint_as_float(ov[k]) * alpha);
+              tc::st16(to + i * 16, ov);
             }
           }
-          const float shift = m == -INFINITY ? 0.0F : -m;
-          const float2 c2 = make_float2(c, c);
-          const float2 shift2 = make_float2(shift, shift);
-          uint32_t ph[16], pl[16];
-          const auto compute = [&](const uint32_t(&v)[32]) {
+        }
+        const float shift = m == -INFINITY ? 0.0F : -m;
+        const float2 c2 = make_float2(c, c);
+        const float2 shift2 = make_float2(shift, shift);
+        uint32_t ph[16], pl[16];
+        const auto compute = [&](const uint32_t(&v)[32]) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float2 p = fma2(make_float2(__uint_as_float(v[2 * i]),
-                                          __uint_as_float(v[2 * i + 1])),
-                              c2, shift2);
-              if (!EDGE && TERMS == 1 && i % 4 == 3) {
-                p = ex2_poly(p);
-              } else {
-                p.x = ex2(p.x);
-                p.y = ex2(p.y);
-              }
-              if (i % 2)
-                sum1 = add2(sum1, p);
-              else
-                sum0 = add2(sum0, p);
-              ph[i] = half2_bits(p.x, p.y);
-              if constexpr (TERMS == 2) {
-                const float2 back = bits_half2(ph[i]);
-                pl[i] = half2_bits(p.x - back.x, p.y - back.y);
-              } else {
-                (void)pl;
-              }
+          for (int i = 0; i < 16; ++i) {
+            float2 p = fma2(make_float2(__uint_as_float(v[2 * i]),
+                                        __uint_as_float(v[2 * i + 1])),
+                            c2, shift2);
+            if (TERMS == 1 && i % 4 == 3) {
+              p = ex2_poly(p);
+            } else {
+              p.x = ex2(p.x);
+              p.y = ex2(p.y);
             }
-          };
-          // P over S: the fp16 terms of keys 32 i .. + 31 take the 32 columns
-          // (16 a term) their scores were read from
-          const auto store = [&](int first) {
-            tc::st16(ts + first, ph);
-            if constexpr (TERMS == 2)
-              tc::st16(ts + first + 16, pl);
-          };
-          const auto arrive = [&](int third) {
-            tc::wait_st();
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0)
-              mbar_arrive(&s.p_full[x][third]);
-          };
-          compute(v0);
-          store(0);
-          tc::ld32(ts + 64, v0);
-          compute(v1);
-          store(32);
-          tc::wait_ld();
-          mask(v0, 64);
-          tc::ld32(ts + 96, v1);
-          compute(v0);
-          arrive(0);
-          store(64);
-          tc::wait_ld();
-          mask(v1, 96);
-          compute(v1);
-          arrive(1);
-          store(96);
-          arrive(2);
+            if (i % 2)
+              sum1 = add2(sum1, p);
+            else
+              sum0 = add2(sum0, p);
+            ph[i] = half2_bits(p.x, p.y);
+            if constexpr (TERMS == 2) {
+              const float2 back = bits_half2(ph[i]);
+              pl[i] = half2_bits(p.x - back.x, p.y - back.y);
+            } else {
+              (void)pl;
+            }
+          }
         };
-        if (range.edge(key0))
-          softmax(std::true_type{});
-        else
-          softmax(std::false_type{});
+        // P over S: the fp16 terms of keys 32 i .. + 31 take the 32 columns
+        // (16 a term) their scores were read from
+        const auto store = [&](int first) {
+          tc::st16(ts + first, ph);
+          if constexpr (TERMS == 2)
+            tc::st16(ts + first + 16, pl);
+        };
+        const auto arrive = [&](int third) {
+          tc::wait_st();
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive(&s.p_full[x][third]);
+        };
+        // (v0 and v1 hold columns 0 .. 63; a piece is handed over once the
+        // next one is worked out, so that its stores need no waiting for)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (half) {
+            tc::wait_ld();
+            mask(v0, 64);
+            tc::ld32(ts + 96, v1);
+          }
+          compute(v0);
+          if (half)
+            arrive(0);
+          store(64 * half);
+          if (half) {
+            tc::wait_ld();
+            mask(v1, 96);
+          } else {
+            tc::ld32(ts + 64, v0);
+          }
+          compute(v1);
+          if (half)
+            arrive(1);
+          store(64 * half + 32);
+        }
+        arrive(2);
       }
       // ---- epilogue
       if (ok)
@@ -701,7 +715,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok)
         break;
       tc::fence_after();
-      const float l = (sum0.x + sum1.x) + (sum0.y + sum1.y);
+      // (a polynomial's 2^-125 of masked keys is not a row's sum)
+      const int seg0 = (g.lo_unit + g.u0) * kChunkKeys;
+      const bool none = own < seg0 || oldest >= seg0 + g.count * kChunkKeys;
+      const float l = none ? 0.0F : (sum0.x + sum1.x) + (sum0.y + sum1.y);
       // (every tile's clearing precedes its P V, which precedes o_full)
       const bool odd = *reinterpret_cast<volatile int*>(&s.odd_values) != 0;
       const bool whole = g.count == g.n_units;
@@ -730,9 +747,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::wait_ld();
         if (odd && live)
           // values that were cleared although this row sees them
-          for (int key = max(oldest, (g.lo_unit + g.u0) * kChunkKeys);
-               key <= min(own, (g.lo_unit + g.u0 + g.count) * kChunkKeys - 1);
-               ++key) {
+          for (int key = max(oldest, seg0);
+               key <= min(own, seg0 + g.count * kChunkKeys - 1); ++key) {
             if (!range.edge(key / kChunkKeys * kChunkKeys))
               continue;  // not a tile that was cleared
             const int pool = paged_row(a.t, a.t.table, g.seq, key);

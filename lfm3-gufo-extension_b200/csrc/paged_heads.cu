@@ -7,11 +7,14 @@
 // HBM bound: every input element is read once and every output written once.
 // A thread moves 16 bytes (4 or 8 elements), so a head is 8 to 32 lanes and a
 // warp takes 1 to 4 heads at a time; the sum of squares and the partner half
-// of each pair come by shuffles inside the head's lanes. A block takes whole
-// rows: its first D / 2 threads turn the row's position into sines and
-// cosines once for all heads. The angle is reduced to half turns in FP64 (at
-// position 10^5 an FP32 product is off by 2^-8 of a radian), the sine and
-// cosine of the remainder are FP32.
+// of each pair come by shuffles inside the head's lanes. Warps are
+// independent: each works on one row, or, when the batch has too few rows to
+// fill the GPU, on a part of its heads (a decode round: one step of heads a
+// warp). The first heads are on their way before the warp knows which sequence
+// its row belongs to. The row's sines and cosines are worked out once for all
+// its heads: angle reduced to half turns in FP64 (at position 10^5 an FP32
+// product is off by 2^-8 of a radian), sine and cosine of the remainder in
+// FP32.
 #include "kernels.cuh"
 #include "paged.cuh"
 
@@ -19,147 +22,162 @@ namespace lfm3 {
 namespace {
 
 constexpr int kHeadsThreads = 256;
-constexpr int kHeadsBlocks = 148 * 8;  // resident blocks of a B200
+constexpr int kHeadsWarps = kHeadsThreads / 32;
+constexpr int kWarpsWanted = 148 * 32;  // warps that fill a B200's SMs
+constexpr int kAhead = 4;               // steps of heads loaded at a time
 
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kHeadsThreads)
-    paged_heads_kernel(const __grid_constant__ PagedHeadsArgs a) {
-  constexpr int kVec = 16 / sizeof(T);        // elements of a thread
-  constexpr int kLanes = DIM / kVec;          // lanes of a head
-  constexpr int kHeadsPerWarp = 32 / kLanes;
+    paged_heads_kernel(const __grid_constant__ PagedHeadsArgs a, int parts) {
+  constexpr int kVec = 16 / sizeof(T);  // elements of a thread
+  constexpr int kLanes = DIM / kVec;    // lanes of a head
+  constexpr int kHeadsPerStep = 32 / kLanes;
   constexpr int kHalf = DIM / 2;
-  __shared__ float cs[kHalf], sn[kHalf];
-  __shared__ int where[3];  // sequence (-1: none), row number, tensor row
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  __shared__ float2 turn[kHeadsWarps][kHalf];  // (cos, sin) of each pair
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int sub = lane / kLanes, part = lane % kLanes;
   const int d0 = part * kVec;  // this thread's first element of the head
   const int kvh = a.t.kv_heads, all = a.heads + 2 * kvh;
-  double turns = 0;  // half turns per position of pair tid
-  if (tid < kHalf) {
-    double f = double(a.freq[tid]);
-    if (a.factors)
-      f /= double(a.factors[tid]);
-    turns = f * 0.31830988618379067154;  // 1 / pi
+  const int steps = (all + kHeadsPerStep - 1) / kHeadsPerStep;
+  grid_dependency_wait();
+  allow_dependents();
+  const int64_t unit = int64_t(blockIdx.x) * kHeadsWarps + warp;
+  if (unit >= int64_t(a.t.rows) * parts)
+    return;
+  const int r = int(unit / parts), first = int(unit - int64_t(r) * parts);
+  // queries, then keys, then values
+  const auto source = [&](int h) -> const T* {
+    if (h < a.heads)
+      return static_cast<const T*>(a.q) + size_t(r) * a.ldq + size_t(h) * DIM;
+    if (h < a.heads + kvh)
+      return static_cast<const T*>(a.k) + size_t(r) * a.ldk +
+             size_t(h - a.heads) * DIM;
+    return static_cast<const T*>(a.v) + size_t(r) * a.ldv +
+           size_t(h - a.heads - kvh) * DIM;
+  };
+  uint4 raw[kAhead];
+  const auto load = [&](int step0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int h = (step0 + i * parts) * kHeadsPerStep + sub;
+      if (h < all)
+        raw[i] = *reinterpret_cast<const uint4*>(source(h) + d0);
+    }
+  };
+  load(first);
+  // ---- the sequence that holds tensor row r
+  int s = -1, number = 0;
+  for (int s0 = 0; s0 < a.t.sequences && s < 0; s0 += 32) {
+    bool hit = false;
+    int row = 0;
+    if (s0 + lane < a.t.sequences) {
+      const PagedSequence q = paged_sequence(a.t, s0 + lane);
+      hit = !q.broken && r >= q.row0 && r < q.row0 + q.n;
+      row = q.length - q.n + (r - q.row0);
+      if (q.broken && unit == 0)
+        report_error(kErrPagedTable);
+    }
+    const unsigned any = __ballot_sync(0xffffffffu, hit);
+    if (any) {
+      s = s0 + __ffs(any) - 1;
+      number = __shfl_sync(0xffffffffu, row, __ffs(any) - 1);
+    }
   }
-  for (int r = blockIdx.x; r < a.t.rows; r += gridDim.x) {
-    if (warp == 0) {
-      // the sequence that holds tensor row r
-      int found = -1, number = 0;
-      for (int s0 = 0; s0 < a.t.sequences && found < 0; s0 += 32) {
-        const int s = s0 + lane;
-        bool hit = false;
-        int row = 0;
-        if (s < a.t.sequences) {
-          const PagedSequence q = paged_sequence(a.t, s);
-          hit = !q.broken && r >= q.row0 && r < q.row0 + q.n;
-          row = q.length - q.n + (r - q.row0);
-          if (q.broken && r == blockIdx.x)
-            report_error(kErrPagedTable);
-        }
-        const unsigned any = __ballot_sync(0xffffffffu, hit);
-        if (any) {
-          found = s0 + __ffs(any) - 1;
-          number = __shfl_sync(0xffffffffu, row, __ffs(any) - 1);
-        }
+  if (s < 0)
+    return;  // not a row of the batch
+  int pool = -1;
+  if (number >= 0) {
+    pool = paged_row(a.t, a.t.table, s, number);
+    if (pool < 0 && lane == 0)
+      report_error(kErrPagedTable);
+  }
+  const int position = a.positions ? a.positions[r] : number;
+#pragma unroll
+  for (int i = lane; i < kHalf; i += 32) {
+    double f = double(a.freq[i]) * 0.31830988618379067154;  // 1 / pi
+    if (a.factors)
+      f /= double(a.factors[i]);
+    const double t = double(position) * f;
+    float sn, cs;
+    sincospif(float(t - 2.0 * rint(t * 0.5)), &sn, &cs);
+    turn[warp][i] = make_float2(cs, sn);
+  }
+  __syncwarp();
+  for (int step0 = first; step0 < steps; step0 += kAhead * parts) {
+    if (step0 != first)
+      load(step0);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int h = (step0 + i * parts) * kHeadsPerStep + sub;
+      if (step0 + i * parts >= steps)
+        break;
+      const bool live = h < all, query = h < a.heads;
+      const bool value = h >= a.heads + kvh;
+      float x[kVec], y[kVec];
+      const T* e = reinterpret_cast<const T*>(&raw[i]);
+      float squares = 0;
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        x[k] = live ? to_float(e[k]) : 0.0F;
+        squares += x[k] * x[k];
       }
-      if (lane == 0) {
-        where[0] = found;
-        where[1] = number;
-        int pool = -1;
-        if (found >= 0 && number >= 0) {
-          pool = paged_row(a.t, a.t.table, found, number);
-          if (pool < 0)
-            report_error(kErrPagedTable);
-        }
-        where[2] = pool;
+#pragma unroll
+      for (int o = kLanes / 2; o; o >>= 1)
+        squares += __shfl_xor_sync(0xffffffffu, squares, o);
+      const float inv = 1.0F / sqrtf(squares * (1.0F / DIM) + a.eps);
+      const float* w = query ? a.q_norm : a.k_norm;
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        const float n = w ? (x[k] * inv) * w[d0 + k] : x[k];
+        const float other = __shfl_xor_sync(0xffffffffu, n, kLanes / 2);
+        const float2 t = turn[warp][(d0 + k) % kHalf];
+        // first half: a cos - b sin; second half: b cos + a sin
+        y[k] = d0 < kHalf ? n * t.x - other * t.y : n * t.x + other * t.y;
       }
-    }
-    __syncthreads();
-    const int s = where[0], pool = where[2];
-    if (s >= 0 && tid < kHalf) {
-      const int position = a.positions ? a.positions[r] : where[1];
-      const double t = double(position) * turns;
-      sincospif(float(t - 2.0 * rint(t * 0.5)), &sn[tid], &cs[tid]);
-    }
-    __syncthreads();
-    if (s >= 0) {
-      for (int h0 = warp * kHeadsPerWarp; h0 < all;
-           h0 += kHeadsThreads / 32 * kHeadsPerWarp) {
-        const int h = h0 + sub;  // queries, then keys, then values
-        const bool live = h < all, query = h < a.heads;
-        const bool value = h >= a.heads + kvh;
-        const int kh = value ? h - a.heads - kvh : h - a.heads;
-        float x[kVec];
+      if (!live)
+        continue;
+      if (query) {
+        alignas(16) T out[kVec];
 #pragma unroll
-        for (int i = 0; i < kVec; ++i)
-          x[i] = 0;
-        if (live) {
-          const T* src =
-              query   ? static_cast<const T*>(a.q) + size_t(r) * a.ldq + size_t(h) * DIM
-              : value ? static_cast<const T*>(a.v) + size_t(r) * a.ldv + size_t(kh) * DIM
-                      : static_cast<const T*>(a.k) + size_t(r) * a.ldk + size_t(kh) * DIM;
-          alignas(16) T raw[kVec];
-          *reinterpret_cast<uint4*>(raw) =
-              *reinterpret_cast<const uint4*>(src + d0);
+        for (int k = 0; k < kVec; ++k)
+          out[k] = from_float<T>(y[k]);
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) +
+                                  size_t(r) * a.ldo + size_t(h) * DIM + d0) =
+            *reinterpret_cast<const uint4*>(out);
+      } else if (pool >= 0) {
+        alignas(16) __half out[kVec];
 #pragma unroll
-          for (int i = 0; i < kVec; ++i)
-            x[i] = to_float(raw[i]);
-        }
-        float y[kVec];
-        const float* w = query ? a.q_norm : a.k_norm;
-        float squares = 0;
-#pragma unroll
-        for (int i = 0; i < kVec; ++i)
-          squares += x[i] * x[i];
-#pragma unroll
-        for (int o = kLanes / 2; o; o >>= 1)
-          squares += __shfl_xor_sync(0xffffffffu, squares, o);
-        const float inv = 1.0F / sqrtf(squares * (1.0F / DIM) + a.eps);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          const float n = w ? (x[i] * inv) * w[d0 + i] : x[i];
-          const float other = __shfl_xor_sync(0xffffffffu, n, kLanes / 2);
-          const int p = (d0 + i) % kHalf;
-          // first half: a cos - b sin; second half: b cos + a sin
-          y[i] = d0 < kHalf ? n * cs[p] - other * sn[p]
-                            : n * cs[p] + other * sn[p];
-        }
-        if (!live)
-          continue;
-        if (query) {
-          alignas(16) T raw[kVec];
-#pragma unroll
-          for (int i = 0; i < kVec; ++i)
-            raw[i] = from_float<T>(y[i]);
-          *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) +
-                                    size_t(r) * a.ldo + size_t(h) * DIM + d0) =
-              *reinterpret_cast<const uint4*>(raw);
-        } else if (pool >= 0) {
-          alignas(16) __half raw[kVec];
-#pragma unroll
-          for (int i = 0; i < kVec; ++i)
-            raw[i] = __float2half_rn(value ? x[i] : y[i]);
-          __half* dst = (value ? a.t.v : a.t.k) +
-                        (size_t(pool) * kvh + kh) * DIM + d0;
-          if constexpr (kVec == 8)
-            *reinterpret_cast<uint4*>(dst) =
-                *reinterpret_cast<const uint4*>(raw);
-          else
-            *reinterpret_cast<uint2*>(dst) =
-                *reinterpret_cast<const uint2*>(raw);
-        }
+        for (int k = 0; k < kVec; ++k)
+          out[k] = __float2half_rn(value ? x[k] : y[k]);
+        __half* dst =
+            (value ? a.t.v : a.t.k) +
+            (size_t(pool) * kvh + (value ? h - a.heads - kvh : h - a.heads)) *
+                DIM + d0;
+        if constexpr (kVec == 8)
+          *reinterpret_cast<uint4*>(dst) =
+              *reinterpret_cast<const uint4*>(out);
+        else
+          *reinterpret_cast<uint2*>(dst) =
+              *reinterpret_cast<const uint2*>(out);
       }
     }
-    __syncthreads();  // where, cs and sn are written again
   }
 }
 
+template <typename T, int DIM>
+cudaError_t launch(const PagedHeadsArgs& a, cudaStream_t stream) {
+  const int per = 32 / (DIM * int(sizeof(T)) / 16);
+  const int steps = (a.heads + 2 * a.t.kv_heads + per - 1) / per;
+  int parts = (kWarpsWanted + a.t.rows - 1) / a.t.rows;
+  parts = parts < steps ? parts : steps;
+  const int64_t warps = int64_t(a.t.rows) * parts;
+  const int64_t blocks = (warps + kHeadsWarps - 1) / kHeadsWarps;
+  return launch_kernel(paged_heads_kernel<T, DIM>, dim3(unsigned(blocks)),
+                       dim3(kHeadsThreads), 0, stream, true, a, parts);
+}
 template <typename T>
 cudaError_t launch(const PagedHeadsArgs& a, int dim, cudaStream_t stream) {
-  const dim3 grid(a.t.rows < kHeadsBlocks ? a.t.rows : kHeadsBlocks);
-  return launch_kernel(dim == 64 ? paged_heads_kernel<T, 64>
-                                 : paged_heads_kernel<T, 128>,
-                       grid, dim3(kHeadsThreads), 0, stream, false, a);
+  return dim == 64 ? launch<T, 64>(a, stream) : launch<T, 128>(a, stream);
 }
 
 }  // namespace
