@@ -147,6 +147,18 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const void* map, int x0,
       : "memory");
 }
 
+// One tiled TMA copy of a 5-D box at (x0, .., x4) of `map`.
+__device__ __forceinline__ void tma_load_5d(void* dst, const void* map, int x0,
+                                            int x1, int x2, int x3, int x4,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_"
+      "tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x0), "r"(x1), "r"(x2), "r"(x3),
+      "r"(x4), "r"(smem_addr(bar))
+      : "memory");
+}
+
 // One tiled TMA copy of a 2-D box at (x0, x1) of `map`.
 __device__ __forceinline__ void tma_load_2d(void* dst, const void* map, int x0,
                                             int x1, uint64_t* bar) {

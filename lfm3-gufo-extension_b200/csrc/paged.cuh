@@ -143,6 +143,11 @@ cudaError_t launch_paged_attention(const PagedAttentionArgs& a, uint32_t type,
                                    int dim, cudaStream_t stream);
 
 struct PagedKeyWeightsArgs {
+  alignas(64) CUtensorMap kmap;  // keys, boxes of box_rows rows of one slab
+  // the queries' fp16 terms, boxes of one query or a whole column block
+  alignas(64) CUtensorMap qmap1[2];
+  alignas(64) CUtensorMap qmap[2];
+  int box_rows;
   PagedTables t;
   const void* q;
   const float* lse;
@@ -150,6 +155,9 @@ struct PagedKeyWeightsArgs {
   size_t ldq;
   int heads, window;
   void* workspace;
+  __half* terms;    // [term][rows][heads][dim]
+  float2* factors;  // [rows][heads]: score factor, lse in base 2
+  float* part;      // slots of 256 sums, then the records
 };
 size_t paged_key_weights_workspace(const PagedTables& t, int dim, int heads);
 cudaError_t launch_paged_key_weights(const PagedKeyWeightsArgs& a,

@@ -45,10 +45,11 @@ int CheckCache(const lfm3_paged_cache* c) {
     return Unsupported("paged cache: sequences must be 0..4096");
   if (c->pages < 1 || c->table_pages < 1 || c->table_stride < c->table_pages)
     return Invalid("paged cache: pages, table_pages and table_stride");
-  // TMA row coordinates and row numbers are 32-bit; products are 64-bit
-  if (int64_t(c->pages) * c->page_rows > INT_MAX ||
-      int64_t(c->table_pages) * c->page_rows > INT_MAX)
-    return Unsupported("paged cache: more than 2^31 - 1 rows");
+  // TMA row coordinates and row numbers (rounded up to tiles) are 32-bit;
+  // products are 64-bit
+  if (int64_t(c->pages) * c->page_rows > INT_MAX - 4096 ||
+      int64_t(c->table_pages) * c->page_rows > INT_MAX - 4096)
+    return Unsupported("paged cache: more than 2^31 - 4097 rows");
   if (!c->k || !c->v || !c->table || !c->lengths)
     return Invalid("paged cache: NULL array");
   if (!Aligned16(c->k) || !Aligned16(c->v))

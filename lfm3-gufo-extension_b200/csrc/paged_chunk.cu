@@ -66,63 +66,10 @@ struct __align__(1024) ChunkSmem {
   int odd_values;  // a value that is not finite was cleared
 };
 
-__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 bits_half2(uint32_t u) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&u));
-}
 // Whether one of a word's two fp16 values is infinite or NaN.
 __device__ __forceinline__ bool not_finite2(uint32_t u) {
   return (((u & 0x7C007C00u) + 0x04000400u) & 0x80008000u) != 0;
 }
-// Two FP32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
-      "mov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\n"
-      "mov.b64 {%0, %1}, x;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
-      "add.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-// 2^x on the FMA pipe: n = round(x), 2^(x - n) by a polynomial of degree 4
-// (least squares reweighted to equal relative error, 2.6e-6, two bits below
-// the half step of an fp16), n added to the exponent. Takes x up to 15 (NaN
-// and infinities make the row NaN before); below -125 it is 2^-125.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  x.x = fmaxf(x.x, -125.0F);
-  x.y = fmaxf(x.y, -125.0F);
-  const float2 magic = make_float2(12582912.0F, 12582912.0F);  // 1.5 * 2^23
-  const float2 back = make_float2(-12582912.0F, -12582912.0F);
-  const float2 t = add2(x, magic);
-  const float2 n = add2(t, back);
-  const float2 f = fma2(n, make_float2(-1.0F, -1.0F), x);
-  float2 p = make_float2(0x1.3997d4p-7F, 0x1.3997d4p-7F);
-  p = fma2(p, f, make_float2(0x1.ca1442p-5F, 0x1.ca1442p-5F));
-  p = fma2(p, f, make_float2(0x1.ec06dap-3F, 0x1.ec06dap-3F));
-  p = fma2(p, f, make_float2(0x1.62e0dcp-1F, 0x1.62e0dcp-1F));
-  p = fma2(p, f, make_float2(0x1.ffffe8p-1F, 0x1.ffffe8p-1F));
-  return make_float2(
-      __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
-
 // What a pair of row tiles sees: rows are the sequence's new rows q0 .. qlast.
 // Every row sees keys all_lo .. all_hi, some row any_lo .. any_hi.
 struct PairRange {

@@ -88,6 +88,46 @@ __device__ inline int64_t chunk_sequence_units(const PagedSequence& q,
   return sum;
 }
 
+// Attention weights: pairs of 128-key tiles against blocks of columns, a
+// column a (query, head of the group) of one KV head. The line runs over
+// sequences, key pairs, KV heads and column blocks.
+constexpr int kWeightKeys = 256;
+constexpr int kWeightCtas = 148;  // one per SM
+
+// Column blocks (chunk_queries queries each) of key pair `pair` in which some
+// query sees some key, from block `lo`.
+__device__ inline int weight_blocks(const PagedSequence& q, int group,
+                                    int window, int pair, int& lo) {
+  const int base = q.length - q.n, k0 = pair * kWeightKeys;
+  const int k1 = min(k0 + kWeightKeys, q.length) - 1;
+  const int first = max(0, k0 - base);
+  int last = q.n - 1;
+  if (window > 0 && int64_t(k1) + window - 1 - base < last)
+    last = k1 + window - 1 - base;
+  lo = first / chunk_queries(group);
+  return last < first ? 0 : last / chunk_queries(group) - lo + 1;
+}
+__device__ inline int weight_pairs(const PagedSequence& q) {
+  return q.n > 0 ? (q.length + kWeightKeys - 1) / kWeightKeys : 0;
+}
+__device__ inline int64_t weight_sequence_units(const PagedSequence& q,
+                                                int group, int window) {
+  const int pairs = weight_pairs(q), base = q.length - q.n;
+  int64_t sum = 0;
+  int lo, p = 0;
+  if (window == 0) {
+    // pairs that begin no later than the first new row: every block
+    p = base < 0 ? 0 : min(pairs, base / kWeightKeys + 1);
+    if (p > 0)
+      sum = int64_t(p) * weight_blocks(q, group, window, 0, lo);
+  } else if (base >= window) {
+    p = (base - window + 1) / kWeightKeys;  // no row sees the pairs before
+  }
+  for (; p < pairs; ++p)
+    sum += weight_blocks(q, group, window, p, lo);
+  return sum;
+}
+
 __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1)
@@ -219,6 +259,53 @@ __device__ bool chunk_segment(const Line& line, int group, int window,
   return false;
 }
 
+// The same for attention weights: inner units u0 .. u0 + count - 1 of n_units
+// (KV head u / blocks, column block lo + u % blocks) of a pair of key tiles.
+struct WeightSegment {
+  PagedSequence q;
+  int seq, pair;
+  int blocks, lo;
+  int n_units, u0, count;
+  int slot;
+};
+template <typename Line>
+__device__ bool weight_segment(const Line& line, int group, int window,
+                               int64_t at, int64_t end, WeightSegment& g) {
+  const int lane = threadIdx.x % 32, kvh = line.t.kv_heads;
+  int64_t before;
+  if (at >= end || !line.find(unit_div(at, kvh), g.seq, g.q, before))
+    return false;
+  const int pairs = weight_pairs(g.q);
+  int64_t rel = at - before * kvh;
+  for (int p0 = 0; p0 < pairs; p0 += 32) {
+    int lo = 0;
+    const int64_t mine =
+        p0 + lane < pairs
+            ? int64_t(weight_blocks(g.q, group, window, p0 + lane, lo)) * kvh
+            : 0;
+    int64_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o)
+        inc += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, inc > rel);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      rel -= __shfl_sync(0xffffffffu, inc - mine, l);
+      g.pair = p0 + l;
+      g.blocks = weight_blocks(g.q, group, window, g.pair, g.lo);
+      g.n_units = g.blocks * kvh;
+      g.u0 = int(rel);
+      g.count = int(min(int64_t(g.n_units - g.u0), end - at));
+      return true;
+    }
+    rel -= __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return false;
+}
+
 // Units per block for a line of `total` units over `ctas` blocks.
 __device__ __forceinline__ int64_t paged_share(int64_t total, int ctas,
                                                int least) {
@@ -266,6 +353,59 @@ __device__ __forceinline__ float row_scale(float top) {
   if (!(top > 0) || e == 255)
     return 1.0F;
   return __uint_as_float(uint32_t(min(127 + 14 - (e - 127), 254)) << 23);
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 bits_half2(uint32_t u) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
+      "mov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\n"
+      "mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
+      "add.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+// 2^x on the FMA pipe: n = round(x), 2^(x - n) by a polynomial of degree 4
+// (least squares reweighted to equal relative error, 2.6e-6, two bits below
+// the half step of an fp16), n added to the exponent. Takes x up to 15 (NaN
+// and infinities make the row NaN before); below -125 it is 2^-125.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  x.x = fmaxf(x.x, -125.0F);
+  x.y = fmaxf(x.y, -125.0F);
+  const float2 magic = make_float2(12582912.0F, 12582912.0F);  // 1.5 * 2^23
+  const float2 back = make_float2(-12582912.0F, -12582912.0F);
+  const float2 t = add2(x, magic);
+  const float2 n = add2(t, back);
+  const float2 f = fma2(n, make_float2(-1.0F, -1.0F), x);
+  float2 p = make_float2(0x1.3997d4p-7F, 0x1.3997d4p-7F);
+  p = fma2(p, f, make_float2(0x1.ca1442p-5F, 0x1.ca1442p-5F));
+  p = fma2(p, f, make_float2(0x1.ec06dap-3F, 0x1.ec06dap-3F));
+  p = fma2(p, f, make_float2(0x1.62e0dcp-1F, 0x1.62e0dcp-1F));
+  p = fma2(p, f, make_float2(0x1.ffffe8p-1F, 0x1.ffffe8p-1F));
+  return make_float2(
+      __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 }  // namespace lfm3

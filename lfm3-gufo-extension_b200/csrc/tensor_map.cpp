@@ -95,6 +95,29 @@ cudaError_t encode_pool_map(CUtensorMap* map, const void* base, int rows,
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t encode_group_map(CUtensorMap* map, const void* base, int rows,
+                             int kv_heads, int group, int dim, int box_rows) {
+  const EncodeTiled encode = Encoder();
+  if (!encode)
+    return cudaErrorNotSupported;
+  if (rows < 1 || kv_heads < 1 || group < 1 || dim % 64 || box_rows < 1 ||
+      box_rows * group > 256 || reinterpret_cast<uintptr_t>(base) % 16)
+    return cudaErrorInvalidValue;
+  const cuuint64_t head = cuuint64_t(dim) * 2;
+  const cuuint64_t dims[5] = {64, cuuint64_t(group), cuuint64_t(rows),
+                              cuuint64_t(dim) / 64, cuuint64_t(kv_heads)};
+  const cuuint64_t strides[4] = {head, head * group * kv_heads, 128,
+                                 head * group};
+  const cuuint32_t box[5] = {64, cuuint32_t(group), cuuint32_t(box_rows), 1, 1};
+  const cuuint32_t element_strides[5] = {1, 1, 1, 1, 1};
+  const CUresult r = encode(
+      map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims,
+      strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 namespace {
 // kind, base, size, rows, box width, box rows
 using MapKey = std::tuple<int, const void*, size_t, int, int, int>;

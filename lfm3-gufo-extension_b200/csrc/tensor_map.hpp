@@ -30,6 +30,13 @@ cudaError_t encode_activation_map(CUtensorMap* map, const void* base, int rows,
 cudaError_t encode_pool_map(CUtensorMap* map, const void* base, int rows,
                             int heads, int dim, int box_rows, int box_slabs);
 
+// Encodes a map over fp16 rows [rows][kv_heads][group][dim] as [kv_heads]
+// [dim / 64][rows][group][64] with boxes of box_rows rows of one KV head and
+// slab, 128-byte swizzle: one copy lands a KV head's (row, head) pairs as
+// 128-byte rows. Box coordinates: 0, 0, row, slab, KV head.
+cudaError_t encode_group_map(CUtensorMap* map, const void* base, int rows,
+                             int kv_heads, int group, int dim, int box_rows);
+
 // The weight and activation maps from a process-wide cache keyed by every
 // encode argument (a hit is exactly the map the encoder would write).
 cudaError_t cached_q8_rows(CUtensorMap* map, const void* base, size_t row_bytes,
