@@ -93,6 +93,49 @@ __device__ __forceinline__ __nv_bfloat16 from_float(float v) {
   return __float2bfloat16_rn(v);
 }
 
+// The elements of 16 bytes, and back (one rounding).
+__device__ __forceinline__ void unpack16(uint4 u, float (&x)[4], float) {
+  x[0] = __uint_as_float(u.x);
+  x[1] = __uint_as_float(u.y);
+  x[2] = __uint_as_float(u.z);
+  x[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void unpack16(uint4 u, float (&x)[8], __half) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void unpack16(uint4 u, float (&x)[8],
+                                         __nv_bfloat16) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint4 pack16(const float (&x)[4], float) {
+  return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]),
+                    __float_as_uint(x[2]), __float_as_uint(x[3]));
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float (&x)[8], T t) {
+  return make_uint4(pack2(x[0], x[1], t), pack2(x[2], x[3], t),
+                    pack2(x[4], x[5], t), pack2(x[6], x[7], t));
+}
+
 struct PagedHeadsArgs {
   PagedTables t;
   const int32_t* positions;

@@ -4,6 +4,9 @@
 //   y = x / sqrt(mean(x^2) + eps) * w
 //   (y_i, y_{i + D/2}) turned by position * f_i / c_i,  i < D / 2
 //
+// An output is then inv (x_i A_i + x_j B_i) with j the partner's place and A_i
+// = w_i cos, B_i = -+ w_j sin constants of the row: the partner's raw value is
+// all that crosses lanes.
 // HBM bound: every input element is read once and every output written once.
 // A thread moves 16 bytes (4 or 8 elements), so a head is 8 to 32 lanes and a
 // warp takes 1 to 4 heads at a time; the sum of squares and the partner half
@@ -40,8 +43,11 @@ __global__ void __launch_bounds__(kHeadsThreads, kBlocksPerSm)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int sub = lane / kLanes, part = lane % kLanes;
   const int d0 = part * kVec;  // this thread's first element of the head
-  const int kvh = a.t.kv_heads, all = a.heads + 2 * kvh;
-  const int steps = (all + kHeadsPerStep - 1) / kHeadsPerStep;
+  const int kvh = a.t.kv_heads;
+  // steps of heads: queries, then keys, then values
+  const int q_steps = (a.heads + kHeadsPerStep - 1) / kHeadsPerStep;
+  const int kv_steps = (kvh + kHeadsPerStep - 1) / kHeadsPerStep;
+  const int steps = q_steps + 2 * kv_steps;
   grid_dependency_wait();
   allow_dependents();
   const int64_t units = int64_t(a.t.rows) * parts;
@@ -51,21 +57,24 @@ __global__ void __launch_bounds__(kHeadsThreads, kBlocksPerSm)
     return;
   int r, first;  // the warp's row, and which of its parts
   uint4 raw[kAhead];
+  // step's kind (0 queries, 1 keys, 2 values) and this lane's head of it
+  const auto kind_of = [&](int step) {
+    return step < q_steps ? 0 : step < q_steps + kv_steps ? 1 : 2;
+  };
+  const auto head_of = [&](int step, int kind) {
+    return (step - (kind ? q_steps : 0) - (kind == 2 ? kv_steps : 0)) *
+               kHeadsPerStep + sub;
+  };
   const auto load = [&](int step0) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int h = (step0 + i * parts) * kHeadsPerStep + sub;
-      // queries, then keys, then values
-      const T* src =
-          h < a.heads ? static_cast<const T*>(a.q) + size_t(r) * a.ldq +
-                            size_t(h) * DIM
-          : h < a.heads + kvh
-              ? static_cast<const T*>(a.k) + size_t(r) * a.ldk +
-                    size_t(h - a.heads) * DIM
-              : static_cast<const T*>(a.v) + size_t(r) * a.ldv +
-                    size_t(h - a.heads - kvh) * DIM;
-      if (h < all)
-        raw[i] = *reinterpret_cast<const uint4*>(src + d0);
+      const int step = step0 + i * parts, kind = kind_of(step);
+      const int h = head_of(step, kind);
+      const void* base = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+      const size_t ld = kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv;
+      if (step < steps && h < (kind ? kvh : a.heads))
+        raw[i] = *reinterpret_cast<const uint4*>(
+            static_cast<const T*>(base) + size_t(r) * ld + h * DIM + d0);
     }
   };
   const auto begin = [&]() {
@@ -89,10 +98,9 @@ __global__ void __launch_bounds__(kHeadsThreads, kBlocksPerSm)
     if (a.factors)
       turns[i] /= double(a.factors[lane + 32 * i]);
   }
-  float wq[kVec];
-#pragma unroll
-  for (int k = 0; k < kVec; ++k)
-    wq[k] = a.q_norm ? a.q_norm[d0 + k] : 1.0F;
+  // norm weights of this lane's elements and of their partners
+  const int other = (d0 + kHalf) % DIM;
+  const float sign = d0 < kHalf ? -1.0F : 1.0F;
 
   for (;;) {
     // ---- the sequence that holds tensor row r
@@ -131,78 +139,67 @@ __global__ void __launch_bounds__(kHeadsThreads, kBlocksPerSm)
         turn[warp][lane + 32 * i] = make_float2(cs, sn);
       }
       __syncwarp();
-      float cs[kVec], sn[kVec];  // of this lane's pairs; + for the second half
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        const float2 t = turn[warp][(d0 + k) % kHalf];
-        cs[k] = t.x;
-        sn[k] = d0 < kHalf ? -t.y : t.y;
-      }
-      __syncwarp();
+      float fa[kVec], fb[kVec];  // A and B of this lane's elements
+      int factors_of = -1;
+      T* const q_out = static_cast<T*>(a.q_out) + size_t(r) * a.ldo + d0;
+      const size_t page_row = size_t(max(pool, 0)) * kvh * DIM + d0;
       for (int step0 = first; step0 < steps; step0 += kAhead * parts) {
         if (step0 != first)
           load(step0);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-          if (step0 + i * parts >= steps)
-            break;
-          const int h = (step0 + i * parts) * kHeadsPerStep + sub;
-          const bool live = h < all, query = h < a.heads;
-          const bool value = h >= a.heads + kvh;
-          const T* e = reinterpret_cast<const T*>(&raw[i]);
-          float x[kVec], y[kVec];
-          float squares = 0;
-#pragma unroll
-          for (int k = 0; k < kVec; ++k) {
-            x[k] = live ? to_float(e[k]) : 0.0F;
-            squares += x[k] * x[k];
-          }
-#pragma unroll
-          for (int o = kLanes / 2; o; o >>= 1)
-            squares += __shfl_xor_sync(0xffffffffu, squares, o);
-          const bool norm = query ? a.q_norm != nullptr : a.k_norm != nullptr;
-          const float inv =
-              norm ? 1.0F / sqrtf(squares * (1.0F / DIM) + a.eps) : 1.0F;
-#pragma unroll
-          for (int k = 0; k < kVec; ++k) {
-            const float w = query  ? wq[k]
-                            : norm ? a.k_norm[d0 + k]
-                                   : 1.0F;
-            const float n = (x[k] * inv) * w;
-            const float other = __shfl_xor_sync(0xffffffffu, n, kLanes / 2);
-            // first half: a cos - b sin; second half: b cos + a sin
-            y[k] = n * cs[k] + other * sn[k];
-          }
-          if (!live)
+          const int step = step0 + i * parts, kind = kind_of(step);
+          const int h = head_of(step, kind);
+          const bool live = h < (kind ? kvh : a.heads);
+          const float* w = kind ? a.k_norm : a.q_norm;
+          if (step >= steps)
             continue;
-          if (query) {
-            alignas(16) T out[kVec];
+          float x[kVec];
+          unpack16(raw[i], x, T{});
+          if (kind < 2) {
+            if (kind != factors_of) {
+              factors_of = kind;
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) {
+                const float2 t = turn[warp][(d0 + k) % kHalf];
+                fa[k] = w ? w[d0 + k] * t.x : t.x;
+                fb[k] = sign * (w ? w[other + k] * t.y : t.y);
+              }
+            }
+            uint4 across;
+            across.x = __shfl_xor_sync(0xffffffffu, raw[i].x, kLanes / 2);
+            across.y = __shfl_xor_sync(0xffffffffu, raw[i].y, kLanes / 2);
+            across.z = __shfl_xor_sync(0xffffffffu, raw[i].z, kLanes / 2);
+            across.w = __shfl_xor_sync(0xffffffffu, raw[i].w, kLanes / 2);
+            float o[kVec], squares = 0;
+            unpack16(across, o, T{});
 #pragma unroll
             for (int k = 0; k < kVec; ++k)
-              out[k] = from_float<T>(y[k]);
-            *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) +
-                                      size_t(r) * a.ldo + size_t(h) * DIM +
-                                      d0) =
-                *reinterpret_cast<const uint4*>(out);
-          } else if (pool >= 0) {
-            alignas(16) __half out[kVec];
+              squares += x[k] * x[k];
+#pragma unroll
+            for (int n = kLanes / 2; n; n >>= 1)
+              squares += __shfl_xor_sync(0xffffffffu, squares, n);
+            const float inv =
+                w ? rsqrtf(squares * (1.0F / DIM) + a.eps) : 1.0F;
 #pragma unroll
             for (int k = 0; k < kVec; ++k)
-              out[k] = __float2half_rn(value ? x[k] : y[k]);
-            __half* dst = (value ? a.t.v : a.t.k) +
-                          (size_t(pool) * kvh +
-                           (value ? h - a.heads - kvh : h - a.heads)) *
-                              DIM +
-                          d0;
+              x[k] = inv * (x[k] * fa[k] + o[k] * fb[k]);
+          }
+          if (kind == 0) {
+            if (live)
+              *reinterpret_cast<uint4*>(q_out + h * DIM) = pack16(x, T{});
+          } else if (live && pool >= 0) {
+            __half* dst = (kind == 1 ? a.t.k : a.t.v) + page_row + h * DIM;
             if constexpr (kVec == 8)
-              *reinterpret_cast<uint4*>(dst) =
-                  *reinterpret_cast<const uint4*>(out);
+              *reinterpret_cast<uint4*>(dst) = pack16(x, __half{});
             else
               *reinterpret_cast<uint2*>(dst) =
-                  *reinterpret_cast<const uint2*>(out);
+                  make_uint2(pack2(x[0], x[1], __half{}),
+                             pack2(x[2], x[3], __half{}));
           }
         }
       }
+      __syncwarp();  // turn is written again
     }
     unit += stride;
     if (unit >= units)
@@ -214,7 +211,8 @@ __global__ void __launch_bounds__(kHeadsThreads, kBlocksPerSm)
 template <typename T, int DIM>
 cudaError_t launch(const PagedHeadsArgs& a, cudaStream_t stream) {
   const int per = 32 / (DIM * int(sizeof(T)) / 16);
-  const int steps = (a.heads + 2 * a.t.kv_heads + per - 1) / per;
+  const int steps = (a.heads + per - 1) / per +
+                    2 * ((a.t.kv_heads + per - 1) / per);
   int parts = (kWarpsWanted + a.t.rows - 1) / a.t.rows;
   parts = parts < steps ? parts : steps;
   const int64_t warps = int64_t(a.t.rows) * parts;
