@@ -11,6 +11,16 @@
 namespace lfm3 {
 namespace {
 
+// Two partial rows (maximum, sum) as one; a sum without a maximum is 0, or
+// NaN, which has to stay. Returns the factors of their outputs.
+__device__ __forceinline__ float2 merge(float2& a, float2 b) {
+  const float m = fmaxf(a.x, b.x);
+  const float fa = a.x == -INFINITY ? 1.0F : ex2(a.x - m);
+  const float fb = b.x == -INFINITY ? 1.0F : ex2(b.x - m);
+  a = make_float2(m, a.y * fa + b.y * fb);
+  return make_float2(fa, fb);
+}
+
 // Merges the stretches that several blocks shared, one record a time: blocks
 // 0 .. 295 (with `decode`) a single token's G heads, then eight blocks a chunk
 // record, 32 of its 256 rows each. Slots add up in key order.
@@ -23,9 +33,8 @@ __global__ void __launch_bounds__(kCombineThreads)
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int kvh = a.t.kv_heads, group = a.heads / kvh;
   __shared__ float tile[kCombineRows][DIM + 4];
-  __shared__ float4 row_scales[kCombineRows];
+  __shared__ float2 row_scales[kCombineRows];  // maximum, factor
   allow_dependents();
-  grid_dependency_wait();
   const bool single = blockIdx.x < decode;
   const int chunk = (blockIdx.x - decode) / (2 * kChunkRows / kCombineRows);
   const float* part = single ? a.decode_part : a.chunk_part;
@@ -33,81 +42,121 @@ __global__ void __launch_bounds__(kCombineThreads)
   const int slots = 2 * (single ? kDecodeCtas : kChunkCtas);
   const float2* pm =
       reinterpret_cast<const float2*>(part + size_t(slots) * rows * DIM);
-  const PagedRecord rec = reinterpret_cast<const PagedRecord*>(
-      pm + size_t(slots) * rows)[single ? blockIdx.x : chunk];
+  grid_dependency_wait();
+  PagedRecord rec;
+  {
+    const int2* r = reinterpret_cast<const int2*>(pm + size_t(slots) * rows) +
+                    (single ? blockIdx.x : chunk) * (sizeof(PagedRecord) / 8);
+    const int2 r0 = __ldcg(r), r1 = __ldcg(r + 1), r2 = __ldcg(r + 2);
+    rec = {r0.x, r0.y, r1.x, r1.y, r2.x, r2.y};
+  }
   if (rec.parts == 0)
     return;
-  // rows of the slot this block merges
-  const int first = single ? 0
-                           : (blockIdx.x - decode) %
-                                 (2 * kChunkRows / kCombineRows) * kCombineRows;
-  const int count = single ? group : kCombineRows;
-  // tensor row and head of slot row i
-  const int QB = chunk_queries(group);
-  const auto place = [&](int i, int& row, int& head) {
-    if (single) {
-      row = rec.row0;
-      head = rec.h * group + i;
-      return true;
+  if (single) {
+    // a warp a head, a lane four dimensions; a few slots at a time, all of
+    // their loads in flight
+    constexpr int kAhead = 8;
+    for (int j = warp; j < group; j += kCombineThreads / 32) {
+      const float* src = part + size_t(j) * DIM + lane % (DIM / 4) * 4;
+      float2 ml = make_float2(-INFINITY, 0);
+      float4 o = make_float4(0, 0, 0, 0);
+      for (int p0 = 0; p0 < rec.parts; p0 += kAhead) {
+        float4 v[kAhead];
+        float2 b[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int sl = record_slot(rec, min(p0 + k, rec.parts - 1));
+          b[k] = __ldcg(pm + sl * rows + j);
+          v[k] = __ldcg(
+              reinterpret_cast<const float4*>(src + size_t(sl) * rows * DIM));
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          if (p0 + k >= rec.parts)
+            break;
+          const float2 f = merge(ml, b[k]);
+          o.x = o.x * f.x + v[k].x * f.y;
+          o.y = o.y * f.x + v[k].y * f.y;
+          o.z = o.z * f.x + v[k].z * f.y;
+          o.w = o.w * f.x + v[k].w * f.y;
+        }
+      }
+      const int head = rec.h * group + j;
+      float scale = 1.0F / ml.y;
+      if (a.gate)
+        scale /= 1 + expf(-to_float(static_cast<const T*>(
+                         a.gate)[size_t(rec.row0) * a.ldg + head]));
+      T* out = static_cast<T*>(a.out) + size_t(rec.row0) * a.ldo +
+               size_t(head) * DIM + lane * 4;
+      if (lane < DIM / 4) {
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<float4*>(out) = make_float4(
+              o.x * scale, o.y * scale, o.z * scale, o.w * scale);
+        else
+          *reinterpret_cast<uint2*>(out) =
+              make_uint2(pack2(o.x * scale, o.y * scale, T{}),
+                         pack2(o.z * scale, o.w * scale, T{}));
+      }
+      if (a.lse && lane == 0)
+        a.lse[size_t(rec.row0) * a.heads + head] =
+            (ml.x + log2f(ml.y)) * kLn2;
     }
+    return;
+  }
+  // ---- a chunk row's maximum, sum and factor: eight threads a row
+  const int first = (blockIdx.x - decode) % (2 * kChunkRows / kCombineRows) *
+                    kCombineRows;
+  const int QB = chunk_queries(group);
+  // tensor row and head of slot row i
+  const auto place = [&](int i, int& row, int& head) {
     const int t = i % kChunkRows;
     const int qi = rec.pair * 2 * QB + i / kChunkRows * QB + t / group;
     row = rec.row0 + qi;
     head = rec.h * group + t % group;
     return t < QB * group && qi < rec.n;
   };
-  // ---- a row's maximum, sum and factor: eight threads a row
-  for (int i0 = 0; i0 < count; i0 += kCombineThreads / 8) {
+  for (int i0 = 0; i0 < kCombineRows; i0 += kCombineThreads / 8) {
     const int i = i0 + tid / 8, sub = tid % 8;
-    float top = -INFINITY, l = 0;
-    if (i < count)
-      for (int p = sub; p < rec.parts; p += 8) {
-        const float2 ml = pm[record_slot(rec, p) * rows + first + i];
-        const float m = fmaxf(top, ml.x);
-        // (a sum without a maximum is 0, or NaN, which has to stay)
-        l = (top == -INFINITY ? l : l * ex2(top - m)) +
-            (ml.x == -INFINITY ? ml.y : ml.y * ex2(ml.x - m));
-        top = m;
-      }
+    float2 ml = make_float2(-INFINITY, 0);
+    for (int p = sub; p < rec.parts; p += 8)
+      merge(ml, __ldcg(pm + record_slot(rec, p) * rows + first + i));
 #pragma unroll
-    for (int o = 4; o; o >>= 1) {
-      const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
-      const float l2 = __shfl_xor_sync(0xffffffffu, l, o);
-      const float m = fmaxf(top, t2);
-      const bool low = (tid & o) == 0;  // both lanes add in the same order
-      const float x = top == -INFINITY ? l : l * ex2(top - m);
-      const float y = t2 == -INFINITY ? l2 : l2 * ex2(t2 - m);
-      l = low ? x + y : y + x;
-      top = m;
+    for (int o = 1; o < 8; o <<= 1) {
+      float2 lower = ml, upper;
+      upper.x = __shfl_xor_sync(0xffffffffu, ml.x, o);
+      upper.y = __shfl_xor_sync(0xffffffffu, ml.y, o);
+      if (sub & o) {  // both lanes add in the same order
+        const float2 t = lower;
+        lower = upper;
+        upper = t;
+      }
+      merge(lower, upper);
+      ml = lower;
     }
-    if (i < count && sub == 0) {
+    if (sub == 0) {
       int row, head;
       float scale = 0;
       if (place(first + i, row, head)) {
-        scale = l == 0 ? 0.0F : 1.0F / l;
+        const bool empty = ml.y == 0;
+        scale = empty ? 0.0F : 1.0F / ml.y;
         if (a.gate)
           scale /= 1 + expf(-to_float(static_cast<const T*>(
                            a.gate)[size_t(row) * a.ldg + head]));
         if (a.lse)
           a.lse[size_t(row) * a.heads + head] =
-              l == 0 ? -INFINITY : (top + log2f(l)) * kLn2;
+              empty ? -INFINITY : (ml.x + log2f(ml.y)) * kLn2;
       }
-      row_scales[i] = make_float4(top, scale, 0, 0);
+      row_scales[i] = make_float2(ml.x, scale);
     }
   }
   __syncthreads();
-  // ---- the outputs: chunk slots lie [dim / 4][row][4] (lane = row), single
-  // ones [row][dim] (lane = four dimensions)
+  // ---- the outputs: slots lie [dim / 4][row][4] (lane = row)
   constexpr int kQuads = DIM / 4;
-  for (int u = warp; u < (single ? count : kQuads);
-       u += kCombineThreads / 32) {
-    const int i = single ? u : lane, d4 = single ? lane : u;
-    if (d4 >= kQuads)
-      continue;
+  for (int d4 = warp; d4 < kQuads; d4 += kCombineThreads / 32) {
+    const int i = lane;
     const float top = row_scales[i].x;
     const size_t step = size_t(rows) * DIM;
-    const float* src = part + (single ? size_t(i) * DIM + d4 * 4
-                                      : (size_t(d4) * rows + first + i) * 4);
+    const float* src = part + (size_t(d4) * rows + first + i) * 4;
     float4 o = make_float4(0, 0, 0, 0);
     for (int p0 = 0; p0 < rec.parts; p0 += 4) {
       float4 v[4];
@@ -115,10 +164,9 @@ __global__ void __launch_bounds__(kCombineThreads)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int sl = record_slot(rec, min(p0 + k, rec.parts - 1));
-        v[k] = *reinterpret_cast<const float4*>(src + sl * step);
-        const float m = pm[sl * rows + first + i].x;
-        f[k] = p0 + k >= rec.parts ? 0.0F : m == -INFINITY ? 1.0F
-                                                           : ex2(m - top);
+        v[k] = __ldcg(reinterpret_cast<const float4*>(src + sl * step));
+        const float m = __ldcg(&pm[sl * rows + first + i].x);
+        f[k] = m == -INFINITY ? 1.0F : ex2(m - top);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -135,7 +183,7 @@ __global__ void __launch_bounds__(kCombineThreads)
         make_float4(o.x * scale, o.y * scale, o.z * scale, o.w * scale);
   }
   __syncthreads();
-  for (int e = tid; e < count * kQuads; e += kCombineThreads) {
+  for (int e = tid; e < kCombineRows * kQuads; e += kCombineThreads) {
     const int i = e / kQuads, d4 = e % kQuads;
     int row, head;
     if (!place(first + i, row, head))
@@ -143,13 +191,11 @@ __global__ void __launch_bounds__(kCombineThreads)
     const float4 y = *reinterpret_cast<const float4*>(&tile[i][d4 * 4]);
     T* out = static_cast<T*>(a.out) + size_t(row) * a.ldo +
              size_t(head) * DIM + d4 * 4;
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4)
       *reinterpret_cast<float4*>(out) = y;
-    } else {
-      alignas(8) T z[4] = {from_float<T>(y.x), from_float<T>(y.y),
-                           from_float<T>(y.z), from_float<T>(y.w)};
-      *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(z);
-    }
+    else
+      *reinterpret_cast<uint2*>(out) =
+          make_uint2(pack2(y.x, y.y, T{}), pack2(y.z, y.w, T{}));
   }
 }
 

@@ -103,14 +103,18 @@ __global__ void __launch_bounds__(kThreads, 2)
   // start once every block is past this point
   grid_dependency_wait();
   allow_dependents();
+  const DecodePlan plan = decode_plan(a.t, group, a.window);
+  const auto rounded = [&](int units) {
+    return (units + plan.pad - 1) / plan.pad * plan.pad;
+  };
   const auto units = [&](const PagedSequence& q) {
-    return int64_t(decode_units(q, group, a.window));
+    return int64_t(rounded(decode_units(q, group, a.window)));
   };
   const PagedLine line(a.t, units);
   if (line.broken && blockIdx.x == 0 && warp == 0)
     report_error(kErrPagedTable);
   const int64_t total = line.total * kvh;
-  const int64_t share = paged_share(total, gridDim.x, kDecodeMinUnits);
+  const int64_t share = plan.share;
   const int64_t begin = share * blockIdx.x, end = min(begin + share, total);
   PagedRecord record{0, 0, 0, 0, 0, 0};
   uint32_t used = 0;  // buffers this warp has filled so far
@@ -126,10 +130,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       break;
     const int n_units = paged_units(q, a.window, 0, 0, kDecodeKeys, lo_unit);
     const int64_t rel = at - before * kvh;
-    const int h = int(unit_div(rel, n_units));
-    const int u0 = int(rel - int64_t(h) * n_units);
+    const int stretch = rounded(n_units);
+    const int h = int(unit_div(rel, stretch));
+    const int u0 = int(rel - int64_t(h) * stretch);
     const int count = int(min(int64_t(n_units - u0), end - at));
-    next = at + count;
+    next = at + (u0 + count == n_units ? stretch - u0 : count);
     // ---- the group's queries are on their way while the page ids come
     const int r = q.row0;
     constexpr int kPerWarp = 8 * NT / kWarps;

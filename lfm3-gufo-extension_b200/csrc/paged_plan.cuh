@@ -56,6 +56,20 @@ __host__ __device__ inline int paged_units(const PagedSequence& q, int window,
   return last < first ? 0 : last / keys - lo + 1;
 }
 
+// Single tokens share out their line in one of two ways. Equal shares cross
+// from one stretch (a KV head of a sequence) to the next, and a block pays for
+// each segment (its queries, its first copies, the merge: 3.5 us, the time of
+// kDecodeSegmentUnits units). Rounding every stretch up to a multiple of the
+// share gives a block one segment, at a larger share. The second is taken when
+// it is no slower: short or few sequences (8 rows of 85 to 1995 keys: 9.6 us
+// a launch with crossing shares, 5 us without), while 32 rows of 512 to 32768
+// keys would take 1.7 times as long.
+constexpr int kDecodeSegmentUnits = 10;
+struct DecodePlan {
+  int64_t share;
+  int pad;  // every stretch's units are rounded up to a multiple of this
+};
+
 // Key units of a single-token sequence (0 for every other).
 __device__ inline int decode_units(const PagedSequence& q, int group,
                                    int window) {
@@ -133,6 +147,33 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
   for (int o = 16; o; o >>= 1)
     v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// (warp-wide)
+__device__ inline DecodePlan decode_plan(const PagedTables& t, int group,
+                                         int window) {
+  int64_t units = 0;
+  int stretches = 0;
+  for (int s = threadIdx.x % 32; s < t.sequences; s += 32) {
+    const int n = decode_units(paged_sequence(t, s), group, window);
+    units += n;
+    stretches += n > 0;
+  }
+  units = warp_sum64(units) * t.kv_heads;
+  const int64_t pairs =
+      int64_t(__reduce_add_sync(0xffffffffu, stretches)) * t.kv_heads;
+  const int64_t crossing =
+      max((units + kDecodeCtas - 1) / kDecodeCtas, int64_t(kDecodeMinUnits));
+  if (pairs < kDecodeCtas) {
+    const uint32_t left = uint32_t(kDecodeCtas - pairs);
+    const int64_t padded =
+        units >> 31 ? units / left
+                    : int64_t((uint32_t(units) + left - 1) / left);
+    if (padded <= crossing + kDecodeSegmentUnits)
+      return {max(padded, int64_t(kDecodeMinUnits)),
+              int(max(padded, int64_t(kDecodeMinUnits)))};
+  }
+  return {crossing, 1};
 }
 
 // Quotient of a unit number by a positive count (64-bit division is a long
