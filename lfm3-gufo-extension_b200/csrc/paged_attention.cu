@@ -55,9 +55,14 @@ __global__ void __launch_bounds__(kCombineThreads)
   if (single) {
     // a warp a head, a lane four dimensions; a few slots at a time, all of
     // their loads in flight
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 16;
     for (int j = warp; j < group; j += kCombineThreads / 32) {
       const float* src = part + size_t(j) * DIM + lane % (DIM / 4) * 4;
+      const int head = rec.h * group + j;
+      float gate = INFINITY;
+      if (a.gate)
+        gate = to_float(static_cast<const T*>(
+            a.gate)[size_t(rec.row0) * a.ldg + head]);
       float2 ml = make_float2(-INFINITY, 0);
       float4 o = make_float4(0, 0, 0, 0);
       for (int p0 = 0; p0 < rec.parts; p0 += kAhead) {
@@ -81,11 +86,7 @@ __global__ void __launch_bounds__(kCombineThreads)
           o.w = o.w * f.x + v[k].w * f.y;
         }
       }
-      const int head = rec.h * group + j;
-      float scale = 1.0F / ml.y;
-      if (a.gate)
-        scale /= 1 + expf(-to_float(static_cast<const T*>(
-                         a.gate)[size_t(rec.row0) * a.ldg + head]));
+      const float scale = 1.0F / ml.y / (1 + expf(-gate));
       T* out = static_cast<T*>(a.out) + size_t(rec.row0) * a.ldo +
                size_t(head) * DIM + lane * 4;
       if (lane < DIM / 4) {
