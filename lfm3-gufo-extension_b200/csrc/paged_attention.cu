@@ -24,7 +24,7 @@ __device__ __forceinline__ float2 merge(float2& a, float2 b) {
 // Merges the stretches that several blocks shared, one record a time: blocks
 // 0 .. 295 (with `decode`) a single token's G heads, then eight blocks a chunk
 // record, 32 of its 256 rows each. Slots add up in key order.
-constexpr int kCombineThreads = 128;
+constexpr int kCombineThreads = 512;
 constexpr int kCombineRows = 32;
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kCombineThreads)
@@ -32,11 +32,12 @@ __global__ void __launch_bounds__(kCombineThreads)
                          int decode) {
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int kvh = a.t.kv_heads, group = a.heads / kvh;
+  constexpr int kChunkBlocks = 2 * kChunkRows / kCombineRows;
   __shared__ float tile[kCombineRows][DIM + 4];
   __shared__ float2 row_scales[kCombineRows];  // maximum, factor
   allow_dependents();
   const bool single = blockIdx.x < decode;
-  const int chunk = (blockIdx.x - decode) / (2 * kChunkRows / kCombineRows);
+  const int chunk = (blockIdx.x - decode) / kChunkBlocks;
   const float* part = single ? a.decode_part : a.chunk_part;
   const int rows = single ? group : 2 * kChunkRows;  // of a slot
   const int slots = 2 * (single ? kDecodeCtas : kChunkCtas);
@@ -105,8 +106,7 @@ __global__ void __launch_bounds__(kCombineThreads)
     return;
   }
   // ---- a chunk row's maximum, sum and factor: eight threads a row
-  const int first = (blockIdx.x - decode) % (2 * kChunkRows / kCombineRows) *
-                    kCombineRows;
+  const int first = (blockIdx.x - decode) % kChunkBlocks * kCombineRows;
   const int QB = chunk_queries(group);
   // tensor row and head of slot row i
   const auto place = [&](int i, int& row, int& head) {
@@ -116,8 +116,8 @@ __global__ void __launch_bounds__(kCombineThreads)
     head = rec.h * group + t % group;
     return t < QB * group && qi < rec.n;
   };
-  for (int i0 = 0; i0 < kCombineRows; i0 += kCombineThreads / 8) {
-    const int i = i0 + tid / 8, sub = tid % 8;
+  if (tid < 8 * kCombineRows) {
+    const int i = tid / 8, sub = tid % 8;
     float2 ml = make_float2(-INFINITY, 0);
     for (int p = sub; p < rec.parts; p += 8)
       merge(ml, __ldcg(pm + record_slot(rec, p) * rows + first + i));
@@ -152,31 +152,37 @@ __global__ void __launch_bounds__(kCombineThreads)
   }
   __syncthreads();
   // ---- the outputs: slots lie [dim / 4][row][4] (lane = row)
-  constexpr int kQuads = DIM / 4;
+  constexpr int kQuads = DIM / 4, kAhead = 8;
+#pragma unroll 1
   for (int d4 = warp; d4 < kQuads; d4 += kCombineThreads / 32) {
     const int i = lane;
     const float top = row_scales[i].x;
     const size_t step = size_t(rows) * DIM;
     const float* src = part + (size_t(d4) * rows + first + i) * 4;
     float4 o = make_float4(0, 0, 0, 0);
-    for (int p0 = 0; p0 < rec.parts; p0 += 4) {
-      float4 v[4];
-      float f[4];
+#pragma unroll 1
+    for (int p0 = 0; p0 < rec.parts; p0 += kAhead) {
+      float4 v[kAhead];
+      float f[kAhead];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int sl = record_slot(rec, min(p0 + k, rec.parts - 1));
-        v[k] = __ldcg(reinterpret_cast<const float4*>(src + sl * step));
-        const float m = __ldcg(&pm[sl * rows + first + i].x);
-        f[k] = m == -INFINITY ? 1.0F : ex2(m - top);
+      for (int k = 0; k < kAhead; ++k) {
+        f[k] = 0;
+        v[k] = make_float4(0, 0, 0, 0);
+        if (p0 + k < rec.parts) {
+          const int sl = record_slot(rec, p0 + k);
+          v[k] = __ldcg(reinterpret_cast<const float4*>(src + sl * step));
+          f[k] = __ldcg(&pm[sl * rows + first + i].x);
+        }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kAhead; ++k) {
         if (p0 + k >= rec.parts)
           break;
-        o.x = fmaf(v[k].x, f[k], o.x);
-        o.y = fmaf(v[k].y, f[k], o.y);
-        o.z = fmaf(v[k].z, f[k], o.z);
-        o.w = fmaf(v[k].w, f[k], o.w);
+        const float w = f[k] == -INFINITY ? 1.0F : ex2(f[k] - top);
+        o.x = fmaf(v[k].x, w, o.x);
+        o.y = fmaf(v[k].y, w, o.y);
+        o.z = fmaf(v[k].z, w, o.z);
+        o.w = fmaf(v[k].w, w, o.w);
       }
     }
     const float scale = row_scales[i].y;

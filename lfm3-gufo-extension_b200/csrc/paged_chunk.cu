@@ -15,7 +15,7 @@
 // overwrites its P: tcgen05.mma of one thread run in order.
 // FP32 queries are two fp16 terms (two MMAs for S, two terms of P, which fill
 // the 128 columns of S, two MMAs for O): 22 bits where a 16-bit type has one.
-// Rows are scaled to fp16's range by a power of two first.
+// Rows are scaled to fp16's range by a power of two first, a batch at a time.
 // A row's probabilities are 2^(x - m) with a reference m that trails the
 // running maximum: 2^7 for the maximum when m moves, 2^15 at most before it
 // moves again, so it (and with it O in tensor memory) moves rarely and
@@ -32,6 +32,8 @@
 // 32 rows, a row at a time over the lanes), 8 TMA, 9 tensor memory and (one
 // thread) every MMA, 10 the clearing, 11 works out the segments ahead of the
 // others. Every wait is bounded.
+#include <type_traits>
+
 #include "kernels.cuh"
 #include "paged.cuh"
 #include "paged_plan.cuh"
@@ -70,6 +72,14 @@ struct __align__(1024) ChunkSmem {
 __device__ __forceinline__ bool not_finite2(uint32_t u) {
   return (((u & 0x7C007C00u) + 0x04000400u) & 0x80008000u) != 0;
 }
+__device__ __forceinline__ uint32_t clear_not_finite(uint32_t u) {
+  if ((u & 0x7C00u) == 0x7C00u)
+    u &= 0xFFFF0000u;
+  if ((u & 0x7C000000u) == 0x7C000000u)
+    u &= 0x0000FFFFu;
+  return u;
+}
+
 // What a pair of row tiles sees: rows are the sequence's new rows q0 .. qlast.
 // Every row sees keys all_lo .. all_hi, some row any_lo .. any_hi.
 struct PairRange {
@@ -159,10 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 11) {
     // ---- the block's segments, then one with count 0
-    const auto units = [&](const PagedSequence& q) {
-      return chunk_sequence_units(q, group, a.window);
-    };
-    const PagedLine line(a.t, units);
+    const PagedLine line(a.t, ChunkUnits{group, a.window});
     if (line.broken && blockIdx.x == 0)
       report_error(kErrPagedTable);
     const int64_t total = line.total * kvh;
@@ -259,30 +266,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int key0 = (g.lo_unit + g.u0 + i / 2) * kChunkKeys;
         if (i % 2 && range.edge(key0)) {
           uint8_t* v = s.kv[st];
-          bool odd = false;
-#pragma unroll 8
-          for (int e = lane; e < 128 * kSlabs * 8; e += 32) {
-            const int key = e / (8 * kSlabs), piece = e % (8 * kSlabs);
-            uint4* at16 = reinterpret_cast<uint4*>(
-                v + (piece / 8) * kSlab + tc::sw128_offset(key, piece % 8));
-            uint4 w = *at16;
-            const bool hidden =
-                key0 + key < range.any_lo || key0 + key > range.any_hi;
-            if (hidden) {
-              *at16 = make_uint4(0, 0, 0, 0);
-            } else if (not_finite2(w.x) || not_finite2(w.y) ||
-                       not_finite2(w.z) || not_finite2(w.w)) {
-              odd = true;
-              __half* h = reinterpret_cast<__half*>(&w);
+          // Few instructions: the softmax warps leave this warp few issue
+          // slots. Rows lo .. hi of the tile are seen by some row of the
+          // pair; the others become 0, then one maximum over everything
+          // tells whether a value is not finite. A 16-byte piece's row is its
+          // place by 128 bytes, whatever the swizzle does inside the row.
+          const int lo = min(max(range.any_lo - key0, 0), 128);
+          const int hi = min(range.any_hi - key0, 127);
+          const int hidden = (lo + 127 - hi) * 8;  // pieces a slab
+          for (int e = lane; e < hidden * kSlabs; e += 32) {
+            const int slab = e >= hidden, i = e - slab * hidden;
+            const int at16 = i < lo * 8 ? i : i - lo * 8 + (hi + 1) * 8;
+            *reinterpret_cast<uint4*>(v + slab * kSlab + at16 * 16) =
+                make_uint4(0, 0, 0, 0);
+          }
+          __syncwarp();
+          __half2 top = __float2half2_rn(0.0F);
+          for (int e0 = lane; e0 < 128 * kSlabs * 8; e0 += 256) {
+            uint4 w[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if ((__half_as_ushort(h[k]) & 0x7C00) == 0x7C00)
-                  h[k] = __ushort_as_half(0);
-              *at16 = w;
+            for (int b = 0; b < 8; ++b)
+              w[b] = *reinterpret_cast<const uint4*>(v + (e0 + 32 * b) * 16);
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+              const __half2* h = reinterpret_cast<const __half2*>(&w[b]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                top = __hmax2_nan(top, __habs2(h[k]));
             }
           }
-          if (odd)
-            *reinterpret_cast<volatile int*>(&s.odd_values) = 1;
+          if (__any_sync(0xffffffffu,
+                         not_finite2(*reinterpret_cast<uint32_t*>(&top)))) {
+            for (int e = lane; e < 128 * kSlabs * 8; e += 32) {
+              uint4* at16 = reinterpret_cast<uint4*>(v + e * 16);
+              uint4 w = *at16;
+              w.x = clear_not_finite(w.x);
+              w.y = clear_not_finite(w.y);
+              w.z = clear_not_finite(w.z);
+              w.w = clear_not_finite(w.w);
+              *at16 = w;
+            }
+            if (lane == 0)
+              *reinterpret_cast<volatile int*>(&s.odd_values) = 1;
+          }
           fence_proxy_async();
           __syncwarp();
         }
@@ -415,6 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ts = tmem + lane_base + x * kColS;
     const uint32_t to = tmem + lane_base + kColO + x * 128;
     // rows over the lanes: kRowLanes lanes of 16 bytes hold one row
+    constexpr bool kHalfType = std::is_same_v<T, __half>;
     constexpr int kVec = 16 / sizeof(T), kRowLanes = DIM / kVec;
     constexpr int kRowsAtOnce = 32 / kRowLanes;
     const int sub = lane / kRowLanes, part = lane % kRowLanes;
@@ -447,6 +474,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const size_t offset = row * a.ldq + size_t(head) * DIM;
         const unsigned alive = __ballot_sync(0xffffffffu, live);
         constexpr int kBatch = kRowsAtOnce > 2 ? 32 / kRowsAtOnce : 16;
+        // One power of two brings the batch's rows into fp16's range (none is
+        // needed for fp16 itself): with 29 binades of normal numbers, rows
+        // 2^18 times smaller than the largest still keep their 22 bits.
 #pragma unroll 1
         for (int i0 = 0; i0 < 32; i0 += kBatch * kRowsAtOnce) {
           uint4 raw[kBatch];
@@ -454,34 +484,41 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < kBatch; ++i) {
             const int r = i0 + i * kRowsAtOnce + sub;
             const size_t at =
-                __shfl_sync(0xffffffffu, (unsigned long long)offset, r & 31);
+                __shfl_sync(0xffffffffu, (unsigned long long)offset, r);
             raw[i] = make_uint4(0, 0, 0, 0);
-            if (r < 32 && (alive >> r & 1))
+            if (alive >> r & 1)
               raw[i] = *reinterpret_cast<const uint4*>(
                   static_cast<const T*>(a.q) + at + part * kVec);
           }
+          float scale = 1;
+          if constexpr (!kHalfType) {
+            float top = 0;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+              float v[kVec];
+              unpack16(raw[i], v, T{});
+#pragma unroll
+              for (int k = 0; k < kVec; ++k)
+                top = fmaxf(top, fabsf(v[k]));
+            }
+            scale = row_scale(warp_max(top));
+          }
+          if (lane >= i0 && lane < i0 + kBatch * kRowsAtOnce)
+            c = scale;
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
             const int r = i0 + i * kRowsAtOnce + sub;
-            const T* e = reinterpret_cast<const T*>(&raw[i]);
-            float v[kVec], top = 0;
-#pragma unroll
-            for (int k = 0; k < kVec; ++k) {
-              v[k] = to_float(e[k]);
-              top = fmaxf(top, fabsf(v[k]));
+            const int piece = part * kVec / 8;
+            const uint32_t off =
+                (piece / 8) * kSlab +
+                tc::sw128_offset((warp % 4) * 32 + r, piece % 8);
+            if constexpr (kHalfType) {
+              *reinterpret_cast<uint4*>(s.q[x][0] + off) = raw[i];
+              continue;
             }
-#pragma unroll
-            for (int o = kRowLanes / 2; o; o >>= 1)
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float scale = row_scale(top);
-            // row r's owner is lane r
-            const float got = __shfl_sync(
-                0xffffffffu, scale,
-                (lane - i0 - i * kRowsAtOnce) * kRowLanes & 31);
-            if (lane - i0 - i * kRowsAtOnce >= 0 &&
-                lane - i0 - i * kRowsAtOnce < kRowsAtOnce)
-              c = got;
+            float v[kVec];
             uint32_t hi[kVec / 2], lo[kVec / 2];
+            unpack16(raw[i], v, T{});
 #pragma unroll
             for (int k = 0; k < kVec / 2; ++k) {
               const float v0 = v[2 * k] * scale, v1 = v[2 * k + 1] * scale;
@@ -489,20 +526,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float2 back = bits_half2(hi[k]);
               lo[k] = half2_bits(v0 - back.x, v1 - back.y);
             }
-            if (r < 32) {
-              const int piece = part * kVec / 8;
-              const uint32_t off =
-                  (piece / 8) * kSlab +
-                  tc::sw128_offset((warp % 4) * 32 + r, piece % 8);
-              if constexpr (TERMS == 2) {
-                *reinterpret_cast<uint2*>(s.q[x][0] + off + (part & 1) * 8) =
-                    make_uint2(hi[0], hi[1]);
-                *reinterpret_cast<uint2*>(s.q[x][1] + off + (part & 1) * 8) =
-                    make_uint2(lo[0], lo[1]);
-              } else {
-                *reinterpret_cast<uint4*>(s.q[x][0] + off) =
-                    make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              }
+            if constexpr (TERMS == 2) {
+              *reinterpret_cast<uint2*>(s.q[x][0] + off + (part & 1) * 8) =
+                  make_uint2(hi[0], hi[1]);
+              *reinterpret_cast<uint2*>(s.q[x][1] + off + (part & 1) * 8) =
+                  make_uint2(lo[0], lo[1]);
+            } else {
+              *reinterpret_cast<uint4*>(s.q[x][0] + off) =
+                  make_uint4(hi[0], hi[1], hi[2], hi[3]);
             }
           }
         }

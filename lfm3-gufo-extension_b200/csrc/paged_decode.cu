@@ -104,12 +104,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   grid_dependency_wait();
   allow_dependents();
   const DecodePlan plan = decode_plan(a.t, group, a.window);
-  const auto rounded = [&](int units) {
-    return (units + plan.pad - 1) / plan.pad * plan.pad;
-  };
-  const auto units = [&](const PagedSequence& q) {
-    return int64_t(rounded(decode_units(q, group, a.window)));
-  };
+  const DecodeUnits units{group, a.window, plan.pad};
   const PagedLine line(a.t, units);
   if (line.broken && blockIdx.x == 0 && warp == 0)
     report_error(kErrPagedTable);
@@ -130,7 +125,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       break;
     const int n_units = paged_units(q, a.window, 0, 0, kDecodeKeys, lo_unit);
     const int64_t rel = at - before * kvh;
-    const int stretch = rounded(n_units);
+    const int stretch = units.rounded(n_units);
     const int h = int(unit_div(rel, stretch));
     const int u0 = int(rel - int64_t(h) * stretch);
     const int count = int(min(int64_t(n_units - u0), end - at));

@@ -92,15 +92,20 @@ __device__ inline int chunk_units(const PagedSequence& q, int group,
   return paged_units(q, window, pair * queries,
                      min(q.n, (pair + 1) * queries) - 1, kChunkKeys, lo);
 }
-__device__ inline int64_t chunk_sequence_units(const PagedSequence& q,
-                                               int group, int window) {
-  const int pairs = chunk_pairs(q, group);
-  int64_t sum = 0;
-  int lo;
-  for (int p = 0; p < pairs; ++p)
-    sum += chunk_units(q, group, window, p, lo);
-  return sum;
-}
+// Units of every step-th pair from pair `from` on (per KV head).
+struct ChunkUnits {
+  static constexpr bool kMany = true;
+  int group, window;
+  __device__ int64_t operator()(const PagedSequence& q, int from,
+                                int step) const {
+    const int pairs = chunk_pairs(q, group);
+    int64_t sum = 0;
+    int lo;
+    for (int p = from; p < pairs; p += step)
+      sum += chunk_units(q, group, window, p, lo);
+    return sum;
+  }
+};
 
 // Attention weights: pairs of 128-key tiles against blocks of columns, a
 // column a (query, head of the group) of one KV head. The line runs over
@@ -124,23 +129,27 @@ __device__ inline int weight_blocks(const PagedSequence& q, int group,
 __device__ inline int weight_pairs(const PagedSequence& q) {
   return q.n > 0 ? (q.length + kWeightKeys - 1) / kWeightKeys : 0;
 }
-__device__ inline int64_t weight_sequence_units(const PagedSequence& q,
-                                                int group, int window) {
-  const int pairs = weight_pairs(q), base = q.length - q.n;
-  int64_t sum = 0;
-  int lo, p = 0;
-  if (window == 0) {
-    // pairs that begin no later than the first new row: every block
-    p = base < 0 ? 0 : min(pairs, base / kWeightKeys + 1);
-    if (p > 0)
-      sum = int64_t(p) * weight_blocks(q, group, window, 0, lo);
-  } else if (base >= window) {
-    p = (base - window + 1) / kWeightKeys;  // no row sees the pairs before
+struct WeightUnits {
+  static constexpr bool kMany = true;
+  int group, window;
+  __device__ int64_t operator()(const PagedSequence& q, int from,
+                                int step) const {
+    const int pairs = weight_pairs(q), base = q.length - q.n;
+    int64_t sum = 0;
+    int lo, p = 0;
+    if (window == 0) {
+      // pairs that begin no later than the first new row: every block
+      p = base < 0 ? 0 : min(pairs, base / kWeightKeys + 1);
+      if (p > 0 && from == 0)
+        sum = int64_t(p) * weight_blocks(q, group, window, 0, lo);
+    } else if (base >= window) {
+      p = (base - window + 1) / kWeightKeys;  // no row sees the pairs before
+    }
+    for (p += from; p < pairs; p += step)
+      sum += weight_blocks(q, group, window, p, lo);
+    return sum;
   }
-  for (; p < pairs; ++p)
-    sum += weight_blocks(q, group, window, p, lo);
-  return sum;
-}
+};
 
 __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
 #pragma unroll
@@ -176,15 +185,29 @@ __device__ inline DecodePlan decode_plan(const PagedTables& t, int group,
   return {crossing, 1};
 }
 
+struct DecodeUnits {
+  static constexpr bool kMany = false;
+  int group, window, pad;
+  __device__ int rounded(int units) const {
+    return (units + pad - 1) / pad * pad;
+  }
+  __device__ int64_t operator()(const PagedSequence& q, int, int) const {
+    return rounded(decode_units(q, group, window));
+  }
+};
+
 // Quotient of a unit number by a positive count (64-bit division is a long
 // sequence of instructions, and lines of 2^32 units are rare).
 __device__ __forceinline__ int64_t unit_div(int64_t a, int b) {
   return uint64_t(a) >> 32 ? a / b : int64_t(uint32_t(a) / uint32_t(b));
 }
 
-// The line of units(sequence) of a batch (all members warp-wide). The first
-// 32 sequences' entries stay in registers, a lane each: for batches of up to
-// 32 the tables are read once.
+// The line of a batch (all members warp-wide); units(sequence, from, step) is
+// every step-th part of a sequence's units from part `from` on. The first 32
+// sequences' entries stay in registers, a lane each: for batches of up to 32
+// the tables are read once. Where a sequence has many parts to sum (kMany), few
+// sequences are summed by all lanes together, more a lane each.
+constexpr int kFewSequences = 8;
 template <typename Units>
 struct PagedLine {
   const PagedTables& t;
@@ -198,9 +221,23 @@ struct PagedLine {
       : t(tables), units(u), own{0, 0, 0, false}, own_units(0), total(0),
         broken(false) {
     const int lane = threadIdx.x % 32;
+    if (Units::kMany && t.sequences <= kFewSequences) {
+      if (lane < t.sequences)
+        own = paged_sequence(t, lane);
+      broken = own.broken;
+      for (int s = 0; s < t.sequences; ++s) {
+        const PagedSequence q{0, __shfl_sync(0xffffffffu, own.n, s),
+                              __shfl_sync(0xffffffffu, own.length, s), false};
+        const int64_t n = warp_sum64(units(q, lane, 32));
+        total += n;
+        if (s == lane)
+          own_units = n;
+      }
+      return;
+    }
     for (int s = lane; s < t.sequences; s += 32) {
       const PagedSequence q = paged_sequence(t, s);
-      const int64_t n = units(q);
+      const int64_t n = units(q, 0, 1);
       broken |= q.broken;
       total += n;
       if (s == lane) {
@@ -225,7 +262,7 @@ struct PagedLine {
         u = 0;
         if (s0 + lane < t.sequences) {
           mine = paged_sequence(t, s0 + lane);
-          u = units(mine);
+          u = units(mine, 0, 1);
         }
       }
       int64_t inc = u;
