@@ -307,7 +307,10 @@ int lfm3_sample_host(const float* logits, int rows, int vocab, int ld,
  *
  * A sequence's rows (one cached key and value each) are numbered from 0 in
  * the order of its tokens; row t lies in row t % page_rows of page
- * table[t / page_rows]. Broken tables are not fatal: where starts decrease or
+ * table[t / page_rows]. Sequences may share pages (a common prefix) where a
+ * call only reads them, lfm3_cuda_paged_attention; lfm3_cuda_paged_heads needs
+ * the new rows' pages, _key_weights and _evict all pages unshared (two
+ * sequences' sums or moves would meet in one row). Broken tables are not fatal: where starts decrease or
  * pass `rows`, a sequence has more than max_rows rows, a length lies outside
  * 0 .. table_pages * page_rows or a page id that a call needs outside
  * 0 .. pages - 1, nothing outside the buffers is touched, that sequence's
@@ -339,9 +342,10 @@ typedef struct lfm3_paged_batch {
 
 /* Checks host copies of the arrays the descriptors point to (k, v and
  * positions are not read): LFM3_OK, or LFM3_ERR_INVALID and a message that
- * names the sequence. Host only. */
+ * names the sequence. Without `shared`, a page that two sequences (or one
+ * twice) hold rows in is refused, too. Host only. */
 int lfm3_paged_check(const lfm3_paged_cache* cache,
-                     const lfm3_paged_batch* batch);
+                     const lfm3_paged_batch* batch, int shared);
 
 /* Per-head RMSNorm and rotation of the new rows' queries and keys (the
  * arithmetic of lfm3_cuda_prompt_heads over a ragged batch; a NULL norm
@@ -405,8 +409,9 @@ int lfm3_cuda_paged_key_weights(const lfm3_paged_cache* cache,
  * as largest), `keep` rows in all (0 <= recent <= keep; sequences that hold no
  * more keep all). Kept rows become rows 0, 1, ... in their old order: keys,
  * values and weights move to the pages of out_table (rows of table_stride
- * entries like table: the cache's own table, or pages that no sequence of the
- * call uses; table_pages * page_rows >= keep). out_lengths (may be
+ * entries like table): each sequence's own, in place (out_table may be table,
+ * or hold the same entries), or pages that no sequence of the call holds rows
+ * in; table_pages * page_rows >= keep. out_lengths (may be
  * cache->lengths) gets min(length, keep); kept [sequences][keep] gets each
  * kept row's old number (entries past the new length are left as they are).
  * Keys keep the rotation of their old positions, so later rows go on counting

@@ -112,7 +112,7 @@ def library():
         "lfm3_cuda_decode_project": ([P, I, I, P, I, P, P, P, P], I),
         "lfm3_cuda_batched_quant_gemm_fp32": ([U32, P, P, P, SZ, SZ, SZ, P], I),
         "lfm3_cuda_exact_bf16_gemm_fp32_small_batch": ([P, P, P, SZ, SZ, SZ, P], I),
-        "lfm3_paged_check": ([P, P], I),
+        "lfm3_paged_check": ([P, P, I], I),
         "lfm3_cuda_paged_heads": ([P, P, U32, P, SZ, P, SZ, P, SZ, P, SZ, I, P,
                                    P, P, P, F, P], I),
         "lfm3_cuda_paged_attention_workspace_bytes": ([P, P, I], SZ),

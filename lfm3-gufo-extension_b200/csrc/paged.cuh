@@ -93,6 +93,25 @@ __device__ __forceinline__ __nv_bfloat16 from_float(float v) {
   return __float2bfloat16_rn(v);
 }
 
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
+      "mov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\n"
+      "mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
+      "add.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // The elements of 16 bytes, and back (one rounding).
 __device__ __forceinline__ void unpack16(uint4 u, float (&x)[4], float) {
   x[0] = __uint_as_float(u.x);
@@ -134,6 +153,15 @@ template <typename T>
 __device__ __forceinline__ uint4 pack16(const float (&x)[8], T t) {
   return make_uint4(pack2(x[0], x[1], t), pack2(x[2], x[3], t),
                     pack2(x[4], x[5], t), pack2(x[6], x[7], t));
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
+      "mul.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
 struct PagedHeadsArgs {

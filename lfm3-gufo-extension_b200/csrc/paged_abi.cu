@@ -3,6 +3,8 @@
 #include <climits>
 #include <cmath>
 #include <cstdio>
+#include <memory>
+#include <new>
 
 #include "../../include/lfm3_cuda.h"
 #include "kernels.cuh"
@@ -127,10 +129,14 @@ PagedTables Tables(const lfm3_paged_cache* c, const lfm3_paged_batch* b) {
 extern "C" {
 
 int lfm3_paged_check(const lfm3_paged_cache* cache,
-                     const lfm3_paged_batch* batch) {
+                     const lfm3_paged_batch* batch, int shared) {
   CHECK(CheckCache(cache));
   CHECK(CheckBatch(batch));
   const PagedTables t = Tables(cache, batch);
+  std::unique_ptr<bool[]> held(shared ? nullptr
+                                      : new (std::nothrow) bool[t.pages]());
+  if (!shared && !held)
+    return Invalid("paged check: out of memory");
   char message[128];
   for (int s = 0; s < t.sequences; ++s) {
     const lfm3::PagedSequence q = lfm3::paged_sequence(t, s);
@@ -140,12 +146,17 @@ int lfm3_paged_check(const lfm3_paged_cache* cache,
                t.starts[s + 1], t.lengths[s]);
       return Invalid(message);
     }
-    for (int64_t row = 0; row < q.length; row += t.page_rows)
-      if (lfm3::paged_row(t, t.table, s, int(row)) < 0) {
-        snprintf(message, sizeof message, "paged sequence %d: page of row %d",
-                 s, int(row));
+    for (int64_t row = 0; row < q.length; row += t.page_rows) {
+      const int pool = lfm3::paged_row(t, t.table, s, int(row));
+      const bool twice = pool >= 0 && !shared && held[pool / t.page_rows];
+      if (pool < 0 || twice) {
+        snprintf(message, sizeof message, "paged sequence %d: page of row %d%s",
+                 s, int(row), twice ? " is held already" : "");
         return Invalid(message);
       }
+      if (!shared)
+        held[pool / t.page_rows] = true;
+    }
   }
   return LFM3_OK;
 }

@@ -153,7 +153,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == 9)
     tc::alloc(&s.tmem, kColumns);
-  if (!a.behind_decode)
+  // Behind the decode kernel this grid may start once every block of that one
+  // is past its own wait, so all that came before it has ended. What an SM has
+  // cached from before that may be stale: the fence drops it.
+  if (a.behind_decode)
+    __threadfence();
+  else
     grid_dependency_wait();
   allow_dependents();
   tc::fence_before();

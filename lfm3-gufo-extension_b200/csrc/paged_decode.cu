@@ -27,6 +27,9 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
+// The largest probability so far is 2^7: small ones stay clear of fp16's
+// subnormals.
+constexpr float kTopExponent = 7.0F;
 
 template <int DIM, int NT, int TERMS>
 struct __align__(1024) DecodeSmem {
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          top = fmaxf(mrun[nt][e], top * c[nt][e]);
+          top = fmaxf(mrun[nt][e], fmaf(top, c[nt][e], -kTopExponent));
           alpha[nt][e] = ex2(mrun[nt][e] - top);
           moved |= top > mrun[nt][e];
           mrun[nt][e] = top;

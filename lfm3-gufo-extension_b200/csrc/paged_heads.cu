@@ -65,32 +65,36 @@ __global__ void __launch_bounds__(kHeadsThreads, kBlocksPerSm)
     return (step - (kind ? q_steps : 0) - (kind == 2 ? kv_steps : 0)) *
                kHeadsPerStep + sub;
   };
+  const T *q_row, *k_row, *v_row;  // of row r, from element d0 on
   const auto load = [&](int step0) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int step = step0 + i * parts, kind = kind_of(step);
       const int h = head_of(step, kind);
-      const void* base = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-      const size_t ld = kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv;
+      const T* base = kind == 0 ? q_row : kind == 1 ? k_row : v_row;
       if (step < steps && h < (kind ? kvh : a.heads))
-        raw[i] = *reinterpret_cast<const uint4*>(
-            static_cast<const T*>(base) + size_t(r) * ld + h * DIM + d0);
+        raw[i] = *reinterpret_cast<const uint4*>(base + h * DIM);
     }
   };
   const auto begin = [&]() {
-    r = int(unit / parts);
+    // (with several parts a row, rows are few)
+    r = parts == 1 ? int(unit) : int(uint32_t(unit) / uint32_t(parts));
     first = int(unit - int64_t(r) * parts);
+    q_row = static_cast<const T*>(a.q) + size_t(r) * a.ldq + d0;
+    k_row = static_cast<const T*>(a.k) + size_t(r) * a.ldk + d0;
+    v_row = static_cast<const T*>(a.v) + size_t(r) * a.ldv + d0;
     load(first);
   };
   begin();
   // ---- constants of the warp: the first 32 sequences, a lane each, the
   // pairs' half turns per position, this lane's norm weights
   PagedSequence mine{0, 0, 0, true};
-  if (lane < a.t.sequences) {
+  if (lane < a.t.sequences)
     mine = paged_sequence(a.t, lane);
-    if (mine.broken && unit == 0)
-      report_error(kErrPagedTable);
-  }
+  if (unit == 0)
+    for (int s = lane; s < a.t.sequences; s += 32)
+      if (paged_sequence(a.t, s).broken)
+        report_error(kErrPagedTable);
   double turns[kHalf / 32];
 #pragma unroll
   for (int i = 0; i < kHalf / 32; ++i) {
@@ -109,11 +113,8 @@ __global__ void __launch_bounds__(kHeadsThreads, kBlocksPerSm)
       PagedSequence q = mine;
       if (s0 > 0) {
         q = PagedSequence{0, 0, 0, true};
-        if (s0 + lane < a.t.sequences) {
+        if (s0 + lane < a.t.sequences)
           q = paged_sequence(a.t, s0 + lane);
-          if (q.broken && unit == 0)
-            report_error(kErrPagedTable);
-        }
       }
       const unsigned any = __ballot_sync(
           0xffffffffu, !q.broken && r >= q.row0 && r < q.row0 + q.n);
@@ -171,19 +172,31 @@ __global__ void __launch_bounds__(kHeadsThreads, kBlocksPerSm)
             across.y = __shfl_xor_sync(0xffffffffu, raw[i].y, kLanes / 2);
             across.z = __shfl_xor_sync(0xffffffffu, raw[i].z, kLanes / 2);
             across.w = __shfl_xor_sync(0xffffffffu, raw[i].w, kLanes / 2);
-            float o[kVec], squares = 0;
+            float o[kVec];
             unpack16(across, o, T{});
+            float2 sum2 = make_float2(0, 0);
 #pragma unroll
-            for (int k = 0; k < kVec; ++k)
-              squares += x[k] * x[k];
+            for (int k = 0; k < kVec; k += 2) {
+              const float2 v = make_float2(x[k], x[k + 1]);
+              sum2 = fma2(v, v, sum2);
+            }
+            float squares = sum2.x + sum2.y;
 #pragma unroll
             for (int n = kLanes / 2; n; n >>= 1)
               squares += __shfl_xor_sync(0xffffffffu, squares, n);
             const float inv =
                 w ? rsqrtf(squares * (1.0F / DIM) + a.eps) : 1.0F;
 #pragma unroll
-            for (int k = 0; k < kVec; ++k)
-              x[k] = inv * (x[k] * fa[k] + o[k] * fb[k]);
+            for (int k = 0; k < kVec; k += 2) {
+              const float2 v =
+                  mul2(make_float2(inv, inv),
+                       fma2(make_float2(x[k], x[k + 1]),
+                            make_float2(fa[k], fa[k + 1]),
+                            mul2(make_float2(o[k], o[k + 1]),
+                                 make_float2(fb[k], fb[k + 1]))));
+              x[k] = v.x;
+              x[k + 1] = v.y;
+            }
           }
           if (kind == 0) {
             if (live)

@@ -440,25 +440,6 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 __device__ __forceinline__ float2 bits_half2(uint32_t u) {
   return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
-// Two FP32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
-      "mov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\n"
-      "mov.b64 {%0, %1}, x;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
-      "add.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));

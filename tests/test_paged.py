@@ -89,8 +89,8 @@ def test_batch_refusals(over):
 def test_missing_descriptors():
     lib, c, b = lfm3.library(), cache(), batch()
     at, bt = ctypes.byref(c), ctypes.byref(b)
-    assert lib.lfm3_paged_check(None, bt) == INVALID
-    assert lib.lfm3_paged_check(at, None) == INVALID
+    assert lib.lfm3_paged_check(None, bt, 0) == INVALID
+    assert lib.lfm3_paged_check(at, None, 1) == INVALID
     assert lib.lfm3_cuda_paged_evict(None, P, P, P, P, 8, 2, None) == INVALID
     assert lib.lfm3_cuda_paged_attention_workspace_bytes(None, bt, 4) == 0
     assert lib.lfm3_cuda_paged_key_weights_workspace_bytes(at, None, 4) == 0
@@ -138,7 +138,7 @@ def test_nothing_to_do_needs_no_arrays():
 
 # ---- tables ------------------------------------------------------------------------
 def check(starts, lengths, table, pages=10, page_rows=16, rows=40, max_rows=40,
-          table_pages=None):
+          table_pages=None, shared=0):
     starts = np.array(starts, np.int32)
     lengths = np.array(lengths, np.int32)
     table = np.array(table, np.int32)
@@ -147,7 +147,8 @@ def check(starts, lengths, table, pages=10, page_rows=16, rows=40, max_rows=40,
               table_pages=table_pages or table.shape[1],
               table_stride=table.shape[1])
     b = batch(starts=starts.ctypes.data, rows=rows, max_rows=max_rows)
-    return lfm3.library().lfm3_paged_check(ctypes.byref(c), ctypes.byref(b))
+    return lfm3.library().lfm3_paged_check(ctypes.byref(c), ctypes.byref(b),
+                                           shared)
 
 
 def test_sound_tables():
@@ -156,6 +157,17 @@ def test_sound_tables():
                                               [4, 99, 99]]) == 0
     assert check([3, 4, 5], [0, 0], [[-1], [77]]) == 0
     assert check([0], [], np.zeros((0, 1))) == 0
+
+
+def test_shared_pages():
+    two = ([0, 1, 2], [33, 20], [[4, 5, 6], [4, 7, 4]])  # a common prefix
+    assert check(*two, shared=1) == 0
+    assert check(*two) == INVALID
+    assert b"sequence 1: page of row 0 is held already" in \
+        lfm3.library().lfm3_last_error()
+    assert check([0, 1], [17], [[3, 3]]) == INVALID
+    # entries past the rows held do not count
+    assert check([0, 1, 2], [16, 16], [[4, 5], [5, 4]]) == 0
 
 
 @pytest.mark.parametrize("starts,lengths,table,more", [

@@ -58,7 +58,7 @@ def check_attention(p, window=0, gate=False):
         empty = np.isneginf(want_lse)
         assert (np.isneginf(got_lse[b:e]) == empty).all()
         assert (got[b:e][empty] == 0).all()
-        z = np.abs(got_lse[b:e] - want_lse)[~empty]
+        z = np.abs(got_lse[b:e][~empty] - want_lse[~empty])
         if z.size:
             # (probabilities' roundings enter the sum as relative errors)
             assert z.max() <= rel + 2.0 ** -22 * np.abs(want_lse[~empty]).max()
@@ -188,6 +188,23 @@ def test_infinite_values_in_other_rows_stay_there():
     assert np.isfinite(p.host(lse)).all()
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_infinite_keys_and_queries(kind):
+    """A NaN query spoils its own rows; a NaN key the rows that see it; their
+    weights and nothing else."""
+    p = Paged([70, 1], [500, 300], 8, 2, 128, kind=kind)
+    p.q[5, 128:256] = float("nan")          # row 5, head 1
+    row = 480                               # seen from new row 50 on
+    p.k[int(p.table[0, row // p.page]), row % p.page, 1] = float("nan")
+    out, lse = p.attention()
+    got = p.host(out)[:, :p.heads * p.dim].reshape(p.rows, p.heads, p.dim)
+    bad = np.zeros((p.rows, p.heads), bool)
+    bad[5, 1] = True
+    bad[50:70, 4:] = True                   # the KV head's four heads
+    assert (np.isnan(got).all(2) == bad).all()
+    assert (np.isfinite(got).all(2) == ~bad).all()
+
+
 def test_same_bits_every_time_and_on_another_stream():
     p = Paged([1, 200, 1], [5000, 3000, 40], kind="bf16")
     a, la = p.attention()
@@ -219,6 +236,78 @@ def test_captured_call_reads_tables_afresh():
     assert torch.equal(out[:, :-8], want[:, :-8])
 
 
+def test_sequences_may_share_pages():
+    """A common prefix: three sequences whose first pages are the same."""
+    p = Paged([1, 70, 1], [900, 600, 300], 8, 2, 128, page=64, kind="f16")
+    for s in (1, 2):
+        p.table[s, :4] = p.table[0, :4]
+    p.dtable = torch.from_numpy(p.table).cuda()
+    check_attention(p)
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, each with its own workspace and outputs."""
+    one = Paged([1, 300, 1], [4000, 2000, 70], kind="f32", seed=1)
+    two = Paged([1] * 20, list(range(100, 2100, 100)), kind="bf16", seed=2)
+    want = [x.attention() for x in (one, two)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for t in streams:
+        t.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for i, x in enumerate((one, two)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(x.attention())
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out, lse in got[i]:
+            assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
+
+
+def test_queries_written_just_before():
+    """Mixed batches run two kernels that overlap: both must see queries that
+    the work queued right before the call wrote."""
+    p = Paged([1, 200, 1, 90], [3000, 1500, 70, 400], kind="bf16")
+    a, b = p.q.clone(), torch.randn_like(p.q)
+    want = []
+    for x in (a, b):
+        p.q.copy_(x)
+        torch.cuda.synchronize()
+        want.append(p.attention()[0].clone())
+    torch.cuda.synchronize()
+    got = []
+    for i in range(20):
+        p.q.copy_((a, b)[i % 2])
+        got.append(p.attention()[0])
+    torch.cuda.synchronize()
+    for i in range(20):
+        assert torch.equal(got[i], want[i % 2])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_long_chunk_rows(kind):
+    """Rows whose keys fill hundreds of tiles of one block (where fp16 rows
+    move their sums out of tensor memory): some rows against FP64."""
+    heads, n, length, dim = 8, 4096, 40960, 64
+    p = Paged([n], [length], heads, heads, dim, page=128, kind=kind)
+    out, lse = p.attention()
+    k, v = p.cached(p.k, 0, length), p.cached(p.v, 0, length)
+    for row in (0, 1, 777, 2048, n - 1):
+        q = p.host(p.q[row, :heads * dim]).reshape(heads, dim)
+        own = length - n + row
+        x = np.einsum("hd,thd->ht", q, k[:own + 1]) / np.sqrt(dim)
+        m = x.max(1, keepdims=True)
+        e = np.exp(x - m)
+        want = np.einsum("ht,thd->hd", e / e.sum(1, keepdims=True), v[:own + 1])
+        got = p.host(out[row, :heads * dim]).reshape(heads, dim)
+        off = np.linalg.norm(got - want) / np.linalg.norm(want)
+        # the two half steps, and for fp16 256 tiles' losses in tensor memory
+        # (a step of at most 2^-23 each, 8 a tile)
+        assert off <= HALF_STEP[kind] + 2.0 ** -11 + 2048 * 2.0 ** -23
+        assert np.abs(p.host(lse[row]) - (m[:, 0] + np.log(e.sum(1)))).max() < 1e-4
+    assert broken() == 0
+
+
 # ---- broken tables: nothing faults, the error word says so ---------------------
 @pytest.mark.parametrize("what", ["page", "length", "starts", "max_rows"])
 def test_broken_tables_are_reported(what):
@@ -241,6 +330,48 @@ def test_broken_tables_are_reported(what):
     weights = torch.zeros(p.pages, p.page, device="cuda")
     p.key_weights(lse, weights)
     assert broken() == 6
+    # heads: only pages that hold new rows are needed
+    q = p.q.clone()
+    k = torch.zeros(p.rows, p.kv_stride, dtype=p.q.dtype, device="cuda")
+    freq = torch.ones(p.dim // 2, device="cuda")
+    if what == "page":
+        p.dtable[1, (400 - 1) // p.page] = -5
+    c, b = p.cache(), p.batch()
+    before = p.k.clone()
+    lfm3.check(lfm3.library().lfm3_cuda_paged_heads(
+        ctypes.byref(c), ctypes.byref(b), TYPES["f16"], q.data_ptr(),
+        p.q_stride, k.data_ptr(), p.kv_stride, k.data_ptr(), p.kv_stride,
+        q.data_ptr(), p.q_stride, p.heads, None, None, freq.data_ptr(), None,
+        0.0, p.stream()))
+    assert broken() == 6
+    # nothing but the new rows' places in sound pages was written
+    changed = (p.k != before) & ~(p.k.isnan() & before.isnan())
+    pages = set(changed.flatten(1).any(1).nonzero().flatten().tolist())
+    fine = {int(x) for s in range(3) for x in p.table[s] if 0 <= x < p.pages}
+    assert pages <= fine
+
+
+@pytest.mark.parametrize("what", ["page", "length", "negative"])
+def test_evict_broken_tables(what):
+    p = Paged([0, 0], [500, 400], 4, 2, 64, page=16)
+    p.k, p.v = torch.nan_to_num(p.k), torch.nan_to_num(p.v)
+    if what == "page":
+        p.dtable[1, 3] = p.pages + 5
+    else:
+        p.dlengths[1] = -1 if what == "negative" else p.width * 16 + 1
+    w = torch.rand(p.pages, 16, device="cuda")
+    kept = torch.full((2, 100), -1, dtype=torch.int32, device="cuda")
+    lengths = torch.zeros(2, dtype=torch.int32, device="cuda")
+    host = w.cpu().numpy()
+    c = p.cache()
+    lfm3.check(lfm3.library().lfm3_cuda_paged_evict(
+        ctypes.byref(c), p.dtable.data_ptr(), lengths.data_ptr(), w.data_ptr(),
+        kept.data_ptr(), 100, 10, p.stream()))
+    assert broken() == 6
+    i = np.arange(500)
+    want = expect_kept(host[p.table[0, i // 16], i % 16], 100, 10)
+    assert (kept[0].cpu().numpy() == want).all()
+    assert lengths[1].item() == (100 if what == "page" else 0)
 
 
 # ---- heads -----------------------------------------------------------------------
@@ -482,6 +613,32 @@ def test_evict_shapes(in_place, kv_heads, dim, page):
 
 def test_evict_long():
     run_evict([20000], 5000, 100, True, page=64, seed=9)
+
+
+def test_evict_many_sequences():
+    """A block a sequence, one of them with more rows than it stages."""
+    run_evict([20000] + [30 + i for i in range(80)], 60, 7, True, page=64)
+    run_evict([17] * 149 + [600], 100, 0, False)
+
+
+def test_evict_in_place_through_a_copy_of_the_table():
+    p = Paged([0, 0], [700, 300], 4, 2, 64, page=16)
+    p.k, p.v = torch.nan_to_num(p.k), torch.nan_to_num(p.v)
+    w = torch.rand(p.pages, 16, device="cuda")
+    kept = torch.full((2, 200), -1, dtype=torch.int32, device="cuda")
+    before, host = p.k.clone(), w.cpu().numpy()
+    c = p.cache()
+    lfm3.check(lfm3.library().lfm3_cuda_paged_evict(
+        ctypes.byref(c), p.dtable.clone().data_ptr(), p.dlengths.data_ptr(),
+        w.data_ptr(), kept.data_ptr(), 200, 20, p.stream()))
+    torch.cuda.synchronize()
+    for s, n in enumerate((700, 300)):
+        i, j = np.arange(n), np.arange(200)
+        want = expect_kept(host[p.table[s, i // 16], i % 16], 200, 20)
+        at = torch.from_numpy(p.table[s].astype(np.int64)).cuda()
+        src, dst = torch.from_numpy(want).cuda(), torch.from_numpy(j).cuda()
+        assert torch.equal(p.k[at[dst // 16], dst % 16],
+                           before[at[src // 16], src % 16])
 
 
 def test_evict_weights_of_every_kind():
