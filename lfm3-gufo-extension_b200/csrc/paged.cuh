@@ -155,12 +155,26 @@ __device__ __forceinline__ uint4 pack16(const float (&x)[8], T t) {
                     pack2(x[4], x[5], t), pack2(x[6], x[7], t));
 }
 
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+// Pairs of FP32 values in 64-bit registers.
+using F32x2 = unsigned long long;
+__device__ __forceinline__ F32x2 pair(float a, float b) {
+  F32x2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 both(F32x2 a) {
   float2 d;
-  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n"
-      "mul.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+  return d;
+}
+__device__ __forceinline__ F32x2 fma_pair(F32x2 a, F32x2 b, F32x2 c) {
+  F32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ F32x2 mul_pair(F32x2 a, F32x2 b) {
+  F32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 

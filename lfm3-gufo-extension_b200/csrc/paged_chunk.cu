@@ -47,6 +47,9 @@ constexpr int kThreads = 12 * 32;
 constexpr uint32_t kColS = 128, kColO = 256, kColumns = 512;
 constexpr uint32_t kSlab = 128 * 128;  // bytes of [128 rows][64 dims]
 constexpr int kPlanned = 4;            // segments worked out ahead
+// key tiles in the time that a block's second segment takes beyond its tiles
+template <int TERMS>
+constexpr int kSegmentUnits = TERMS == 2 ? 3 : 6;
 // exponents (base 2) of a row's largest probability: when the reference
 // moves, and when it has to move again
 constexpr float kTopMoved = 7.0F, kTopLimit = 15.0F;
@@ -187,18 +190,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 11) {
     // ---- the block's segments, then one with count 0
-    const PagedLine line(a.t, ChunkUnits{group, a.window});
+    PagedLine<ChunkUnits> line(a.t, ChunkUnits{group, a.window, 1});
+    const int64_t share = chunk_plan(line, kSegmentUnits<TERMS>);
     if (line.broken && blockIdx.x == 0)
       report_error(kErrPagedTable);
     const int64_t total = line.total * kvh;
-    const int64_t share = paged_share(total, kChunkCtas, kChunkMinUnits);
     const int64_t begin = share * blockIdx.x, end = min(begin + share, total);
     PagedRecord record{0, 0, 0, 0, 0, 0};
     int64_t at = begin;
     for (bool more = true; more && ok; ++planned) {
-      more = chunk_segment(line, group, a.window, at, end, g);
+      more = chunk_segment(line, at, end, g);
       if (!more)
-        g.count = 0;
+        g.count = g.units = 0;
       g.slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
       const uint32_t i = planned % kPlanned;
       if (planned >= kPlanned)
@@ -213,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (more && g.count < g.n_units && g.u0 == 0)
         record = paged_record(at, share, g.slot, g.n_units, g.q, g.pair, g.h);
-      at += g.count;
+      at += g.units;
     }
     if (lane == 0)
       reinterpret_cast<PagedRecord*>(
@@ -423,19 +426,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         if (!two)
           tc::commit_lead(&s.kv_empty[vs], lead);
+        // O is whole: at the end, and where it moves out of tensor memory
+        const bool handed = !more || (j + 1) % kFlushTiles<T> == 0;
+        if (handed)
+          tc::commit_lead(&s.o_full[0], lead);
         if (more)
           scores(0, ks);
-        else
-          tc::commit_lead(&s.o_full[0], lead);
         if (two) {
           ok = consume(1, vs, later, (tiles1 + j) & 1);
           if (!ok)
             break;
           tc::commit_lead(&s.kv_empty[vs], lead);
+          if (handed)
+            tc::commit_lead(&s.o_full[1], lead);
           if (more)
             scores(1, ks);
-          else
-            tc::commit_lead(&s.o_full[1], lead);
         }
         if (more) {
           tc::commit_lead(&s.kv_empty[ks], lead);
@@ -470,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const auto wait_all = [&](uint64_t* bar, uint32_t parity) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, kErrPagedWait));
     };
-    uint32_t tiles = 0, segments = 0;
+    uint32_t tiles = 0, segments = 0, o_uses = 0;
     while (next_segment()) {
       const PairRange range(g, QB, a.window);
       if (x == 1 && g.q.n - range.q0 <= QB)
@@ -569,16 +574,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       float2 sum0 = make_float2(0, 0), sum1 = sum0;
       for (int j = 0; j < g.count; ++j) {
         const int key0 = (g.lo_unit + g.u0 + j) * kChunkKeys;
-        if (!wait_all(&s.s_full[x], (tiles + j) & 1)) {
-          ok = false;
-          break;
-        }
-        tc::fence_after();
-        // S is read twice, for the maximum and for the probabilities: with
-        // all 128 values and the packed P live, registers would spill
         const bool flush = j % kFlushTiles<T> == 0;
         if (kCanFlush && flush && j > 0) {
-          // (P_{j-1} V_{j-1} was issued before S_j, which has completed)
+          // while S_j is computed
+          if (!wait_all(&s.o_full[x], o_uses++ & 1)) {
+            ok = false;
+            break;
+          }
+          tc::fence_after();
           // (no reader but this thread: the additions need no answer)
           const bool moved = __any_sync(0xffffffffu, !(m_slot == m));
           const bool first = j == kFlushTiles<T>;
@@ -612,6 +615,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           m_slot = m;
         }
+        if (!wait_all(&s.s_full[x], (tiles + j) & 1)) {
+          ok = false;
+          break;
+        }
+        tc::fence_after();
+        // S is read twice, for the maximum and for the probabilities: with
+        // all 128 values and the packed P live, registers would spill
         const bool edge = range.edge(key0);
         const int hi = own - key0, lo = oldest - key0;
         // columns first .. first + 31 that the row does not see become -inf
@@ -745,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // ---- epilogue
       if (ok)
-        ok = wait_all(&s.o_full[x], segments & 1);
+        ok = wait_all(&s.o_full[x], o_uses++ & 1);
       if (!ok)
         break;
       tc::fence_after();

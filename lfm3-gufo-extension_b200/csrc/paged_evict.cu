@@ -55,13 +55,13 @@ __device__ __forceinline__ uint32_t key_at(const PagedEvictArgs& a, int s,
 }
 
 // Exclusive sum over the block in thread order; *total gets the whole sum.
-__device__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums,
-                               uint32_t* total) {
+template <typename N>
+__device__ N block_scan(N v, N* warp_sums, N* total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  uint32_t inc = v;
+  N inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t t = __shfl_up_sync(0xffffffffu, inc, o);
+    const N t = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o)
       inc += t;
   }
@@ -70,10 +70,10 @@ __device__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums,
     warp_sums[warp] = inc;
   __syncthreads();
   // every warp scans the 32 warps' sums
-  uint32_t w = warp_sums[lane], all = w;
+  N w = warp_sums[lane], all = w;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t t = __shfl_up_sync(0xffffffffu, all, o);
+    const N t = __shfl_up_sync(0xffffffffu, all, o);
     if (lane >= o)
       all += t;
   }
@@ -85,9 +85,10 @@ __global__ void __launch_bounds__(kSelectThreads)
     paged_evict_select_kernel(const __grid_constant__ PagedEvictArgs a) {
   namespace cg = cooperative_groups;
   extern __shared__ uint32_t keys[];  // [kStagedRows]
-  __shared__ uint32_t hist[3][kBins];
-  __shared__ uint32_t sums[kSelectThreads / 32];
+  alignas(16) __shared__ uint32_t hist[3][kBins];
+  __shared__ unsigned long long sums[kSelectThreads / 32];
   __shared__ uint32_t digit, due;
+  __shared__ uint32_t totals[2];  // this block's sure rows, and at threshold
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = cluster.block_rank(), ranks = cluster.num_blocks();
   const int s = blockIdx.x / ranks, tid = threadIdx.x, lane = tid % 32;
@@ -124,7 +125,9 @@ __global__ void __launch_bounds__(kSelectThreads)
     for (int t = row0 + tid; t < mid; t += kSelectThreads)
       keys[t - row0] = key_at(a, s, t);
   }
+  // (the last `recent` rows stay for sure)
   uint32_t prefix = 0, mask = 0, remaining = want;
+  uint32_t own_sure = max(row1 - max(row0, old), 0), own_ties = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 3 && want > 0; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
@@ -150,8 +153,10 @@ __global__ void __launch_bounds__(kSelectThreads)
     }
     cluster.sync();
     // the bin that holds the remaining-th largest: thread i has the two bins
-    // from the top that begin at 2 i
+    // from the top that begin at 2 i. One scan carries the cluster's counts
+    // and this block's own.
     const uint32_t b0 = kBins - 1 - 2 * tid;
+    const uint32_t o0 = hist[pass][b0], o1 = hist[pass][b0 - 1];
     uint32_t h0 = 0, h1 = 0;
 #pragma unroll
     for (int r = 0; r < kSelectCluster; ++r) {
@@ -162,17 +167,24 @@ __global__ void __launch_bounds__(kSelectThreads)
       h1 += h.x;
       h0 += h.y;
     }
-    uint32_t all;
-    const uint32_t above = block_scan(h0 + h1, sums, &all);
+    using Two = unsigned long long;
+    Two all;
+    const Two scan =
+        block_scan<Two>(Two(h0 + h1) << 32 | (o0 + o1), sums, &all);
+    const uint32_t above = uint32_t(scan >> 32);
     if (above < remaining && remaining <= above + h0 + h1) {
       const bool second = remaining > above + h0;
       digit = second ? b0 - 1 : b0;
       due = remaining - above - (second ? h0 : 0);
+      totals[0] = uint32_t(scan) + (second ? o0 : 0);  // of this block, above
+      totals[1] = second ? o1 : o0;
     }
     __syncthreads();
     prefix |= digit << shift;
     mask |= (bins - 1) << shift;
     remaining = due;
+    own_sure += totals[0];
+    own_ties = totals[1];
   }
   // A row stays for sure, or is at the threshold: `remaining` of those stay,
   // the lowest. Bit 2 r: sure, 2 r + 1: at the threshold, of row t0 + r.
@@ -195,22 +207,13 @@ __global__ void __launch_bounds__(kSelectThreads)
   constexpr uint32_t kSureBits = 0x55, kTieBits = 0xAA;
   constexpr int kStep = kSelectThreads * kSelectRows;
   static_assert(kSelectRows == 4, "the masks are of four rows");
-  uint32_t sure = 0, ties = 0;
-  for (int t0 = row0 + tid * kSelectRows; t0 < row1; t0 += kStep) {
-    const uint32_t f = flags_at(t0);
-    sure += __popc(f & kSureBits);
-    ties += __popc(f & kTieBits);
+  __syncthreads();  // the last pass has read totals
+  if (tid == 0) {
+    totals[0] = own_sure;
+    totals[1] = own_ties;
   }
-  __shared__ uint32_t totals[2];
-  uint32_t all;
-  block_scan(sure, sums, &all);
-  if (tid == 0)
-    totals[0] = all;
-  block_scan(ties, sums, &all);
-  if (tid == 0)
-    totals[1] = all;
   cluster.sync();
-  sure = ties = 0;  // rows before this block's
+  uint32_t sure = 0, ties = 0;  // rows before this block's
 #pragma unroll
   for (int r = 0; r < kSelectCluster; ++r)
     if (r < rank) {
@@ -221,9 +224,10 @@ __global__ void __launch_bounds__(kSelectThreads)
   for (int s0 = row0; s0 < row1; s0 += kStep) {
     const int t0 = s0 + tid * kSelectRows;
     const uint32_t flags = flags_at(t0);
-    const uint32_t before =
-        block_scan(__popc(flags & kSureBits) | __popc(flags & kTieBits) << 16,
-                   sums, &all);
+    unsigned long long all;
+    const uint32_t before = uint32_t(block_scan<unsigned long long>(
+        __popc(flags & kSureBits) | __popc(flags & kTieBits) << 16, sums,
+        &all));
     uint32_t at = sure + (before & 0xffffu), tie = ties + (before >> 16);
 #pragma unroll
     for (int r = 0; r < kSelectRows; ++r) {
@@ -236,8 +240,8 @@ __global__ void __launch_bounds__(kSelectThreads)
       at += stays;
       tie += even;
     }
-    sure += all & 0xffffu;
-    ties += all >> 16;
+    sure += uint32_t(all) & 0xffffu;
+    ties += uint32_t(all) >> 16;
   }
   cluster.sync();  // the others have read this block's shared memory
 }
@@ -293,10 +297,10 @@ __device__ void copy_rows(const PagedEvictArgs& a, int s, int count,
 }
 
 // Block (slice, sequence). In place: 16-byte columns [slice * cols, + cols) of
-// the rows of K, then V; the last slice moves the weights.
+// the rows of K, then V; block `slices` moves the weights.
 __global__ void __launch_bounds__(kMoveThreads, 3)
     paged_evict_move_kernel(const __grid_constant__ PagedEvictArgs a,
-                            int row_pieces, int cols) {
+                            int row_pieces, int cols, int slices) {
   const int s = blockIdx.y, tid = threadIdx.x;
   grid_dependency_wait();
   allow_dependents();
@@ -309,7 +313,9 @@ __global__ void __launch_bounds__(kMoveThreads, 3)
     copy_rows(a, s, count, row_pieces);
     return;
   }
-  const bool weights = blockIdx.x == gridDim.x - 1;
+  if (blockIdx.x > slices)
+    return;
+  const bool weights = blockIdx.x == slices;
   const int c = weights ? 1 : cols;
   const int piece = blockIdx.x * cols + tid % c;
   const bool mine = weights || piece < 2 * row_pieces;
@@ -401,16 +407,17 @@ cudaError_t launch_paged_evict(const PagedEvictArgs& a, int dim,
   if ((e = cudaLaunchKernelEx(&config, paged_evict_select_kernel, a)))
     return e;
   const int pieces = a.t.kv_heads * dim / 8;  // 16-byte pieces of a row
-  // Columns of a block: as many (up to 8, 128 bytes) as leave a block for
-  // every SM. One sequence of 8192 kept rows of 2 x 1 KB: 1 column (128
-  // blocks) 12 us, 8 columns (16 blocks) 48 us; 24 sequences of 2000: 8
-  // columns 22 us, 1 column 47 us.
+  // In place, columns of a block: as many (up to 8, 128 bytes) as leave a
+  // block for every SM. Whole rows want 16 warps of an SM.
   int cols = 8;
   while (cols > 1 && (2 * pieces + cols - 1) / cols * a.t.sequences < 148)
     cols /= 2;
-  return launch_kernel(paged_evict_move_kernel,
-                       dim3((2 * pieces + cols - 1) / cols + 1, a.t.sequences),
-                       dim3(kMoveThreads), 0, stream, true, a, pieces, cols);
+  const int slices = (2 * pieces + cols - 1) / cols;
+  const int blocks =
+      std::max(slices + 1, (148 * 2 + a.t.sequences - 1) / a.t.sequences);
+  return launch_kernel(paged_evict_move_kernel, dim3(blocks, a.t.sequences),
+                       dim3(kMoveThreads), 0, stream, true, a, pieces, cols,
+                       slices);
 }
 
 }  // namespace lfm3

@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kHeadsThreads, kBlocksPerSm)
         turn[warp][lane + 32 * i] = make_float2(cs, sn);
       }
       __syncwarp();
-      float fa[kVec], fb[kVec];  // A and B of this lane's elements
+      F32x2 fa[kVec / 2], fb[kVec / 2];  // A and B of this lane's elements
       int factors_of = -1;
       T* const q_out = static_cast<T*>(a.q_out) + size_t(r) * a.ldo + d0;
       const size_t page_row = size_t(max(pool, 0)) * kvh * DIM + d0;
@@ -161,10 +161,15 @@ __global__ void __launch_bounds__(kHeadsThreads, kBlocksPerSm)
             if (kind != factors_of) {
               factors_of = kind;
 #pragma unroll
-              for (int k = 0; k < kVec; ++k) {
-                const float2 t = turn[warp][(d0 + k) % kHalf];
-                fa[k] = w ? w[d0 + k] * t.x : t.x;
-                fb[k] = sign * (w ? w[other + k] * t.y : t.y);
+              for (int k = 0; k < kVec; k += 2) {
+                const float2 t0 = turn[warp][(d0 + k) % kHalf];
+                const float2 t1 = turn[warp][(d0 + k + 1) % kHalf];
+                const float a0 = w ? w[d0 + k] : 1.0F;
+                const float a1 = w ? w[d0 + k + 1] : 1.0F;
+                const float b0 = w ? w[other + k] : 1.0F;
+                const float b1 = w ? w[other + k + 1] : 1.0F;
+                fa[k / 2] = pair(a0 * t0.x, a1 * t1.x);
+                fb[k / 2] = pair(sign * b0 * t0.y, sign * b1 * t1.y);
               }
             }
             uint4 across;
@@ -174,28 +179,27 @@ __global__ void __launch_bounds__(kHeadsThreads, kBlocksPerSm)
             across.w = __shfl_xor_sync(0xffffffffu, raw[i].w, kLanes / 2);
             float o[kVec];
             unpack16(across, o, T{});
-            float2 sum2 = make_float2(0, 0);
+            F32x2 sum2 = pair(0, 0), y[kVec / 2];
 #pragma unroll
-            for (int k = 0; k < kVec; k += 2) {
-              const float2 v = make_float2(x[k], x[k + 1]);
-              sum2 = fma2(v, v, sum2);
+            for (int k = 0; k < kVec / 2; ++k) {
+              const F32x2 v = pair(x[2 * k], x[2 * k + 1]);
+              sum2 = fma_pair(v, v, sum2);
+              y[k] = fma_pair(v, fa[k],
+                              mul_pair(pair(o[2 * k], o[2 * k + 1]), fb[k]));
             }
-            float squares = sum2.x + sum2.y;
+            const float2 sums = both(sum2);
+            float squares = sums.x + sums.y;
 #pragma unroll
             for (int n = kLanes / 2; n; n >>= 1)
               squares += __shfl_xor_sync(0xffffffffu, squares, n);
             const float inv =
                 w ? rsqrtf(squares * (1.0F / DIM) + a.eps) : 1.0F;
+            const F32x2 inv2 = pair(inv, inv);
 #pragma unroll
-            for (int k = 0; k < kVec; k += 2) {
-              const float2 v =
-                  mul2(make_float2(inv, inv),
-                       fma2(make_float2(x[k], x[k + 1]),
-                            make_float2(fa[k], fa[k + 1]),
-                            mul2(make_float2(o[k], o[k + 1]),
-                                 make_float2(fb[k], fb[k + 1]))));
-              x[k] = v.x;
-              x[k + 1] = v.y;
+            for (int k = 0; k < kVec / 2; ++k) {
+              const float2 v = both(mul_pair(y[k], inv2));
+              x[2 * k] = v.x;
+              x[2 * k + 1] = v.y;
             }
           }
           if (kind == 0) {

@@ -92,17 +92,21 @@ __device__ inline int chunk_units(const PagedSequence& q, int group,
   return paged_units(q, window, pair * queries,
                      min(q.n, (pair + 1) * queries) - 1, kChunkKeys, lo);
 }
-// Units of every step-th pair from pair `from` on (per KV head).
+// Units of every step-th pair from pair `from` on (per KV head), each pair's
+// rounded up to a multiple of `pad`.
 struct ChunkUnits {
   static constexpr bool kMany = true;
-  int group, window;
+  int group, window, pad;
+  __device__ int rounded(int units) const {
+    return pad == 1 ? units : (units + pad - 1) / pad * pad;
+  }
   __device__ int64_t operator()(const PagedSequence& q, int from,
                                 int step) const {
     const int pairs = chunk_pairs(q, group);
     int64_t sum = 0;
     int lo;
     for (int p = from; p < pairs; p += step)
-      sum += chunk_units(q, group, window, p, lo);
+      sum += rounded(chunk_units(q, group, window, p, lo));
     return sum;
   }
 };
@@ -225,14 +229,7 @@ struct PagedLine {
       if (lane < t.sequences)
         own = paged_sequence(t, lane);
       broken = own.broken;
-      for (int s = 0; s < t.sequences; ++s) {
-        const PagedSequence q{0, __shfl_sync(0xffffffffu, own.n, s),
-                              __shfl_sync(0xffffffffu, own.length, s), false};
-        const int64_t n = warp_sum64(units(q, lane, 32));
-        total += n;
-        if (s == lane)
-          own_units = n;
-      }
+      reset(u);
       return;
     }
     for (int s = lane; s < t.sequences; s += 32) {
@@ -246,6 +243,20 @@ struct PagedLine {
       }
     }
     total = warp_sum64(total);
+  }
+
+  // The same sequences (at most 32) with other units.
+  __device__ void reset(Units u) {
+    units = u;
+    total = own_units = 0;
+    for (int s = 0; s < t.sequences; ++s) {
+      const PagedSequence q{0, __shfl_sync(0xffffffffu, own.n, s),
+                            __shfl_sync(0xffffffffu, own.length, s), false};
+      const int64_t n = warp_sum64(units(q, threadIdx.x % 32, 32));
+      total += n;
+      if (s == threadIdx.x % 32)
+        own_units = n;
+    }
   }
 
   // The sequence that holds unit `at`, its numbers, and the units before it.
@@ -289,20 +300,66 @@ struct PagedLine {
   }
 };
 
+// Units per block for a line of `total` units over `ctas` blocks.
+__device__ __forceinline__ int64_t paged_share(int64_t total, int ctas,
+                                               int least) {
+  return max((total + ctas - 1) / ctas, int64_t(least));
+}
+
 // One block's next piece of the chunks' line: units u0 .. u0 + count - 1 (of
 // n_units, the first of them key tile `lo_unit`) of a pair of row tiles and a
-// KV head, and the block's slot for it.
+// KV head, `units` of the line with its rounding, and the block's slot for it.
 struct ChunkSegment {
   PagedSequence q;
   int seq, pair, h;
-  int n_units, lo_unit, u0, count;
+  int n_units, lo_unit, u0, count, units;
   int slot;
 };
+// The chunks' share and rounding (warp-wide), the same choice as decode_plan's:
+// when there is a block for every stretch, the smallest share with which the
+// rounded stretches still fit the blocks is taken, unless crossing shares save
+// more than a second segment costs (its queries, its first copies, its
+// epilogue: about 8 us, `segment` tiles). 512 FP32 rows at depth 8192, 32
+// stretches of 65 to 68 tiles: shares of 17 tiles instead of 15, 91 -> 82 us.
+__device__ inline int64_t chunk_plan(PagedLine<ChunkUnits>& line,
+                                     int segment) {
+  const PagedTables& t = line.t;
+  const ChunkUnits& units = line.units;
+  const int lane = threadIdx.x % 32, kvh = t.kv_heads;
+  const int64_t crossing = paged_share(line.total * kvh, kChunkCtas, 1);
+  int stretches = 0;
+  if (lane < t.sequences)
+    stretches = chunk_pairs(line.own, units.group) * kvh;
+  if (t.sequences > 32 || crossing > 1 << 20 ||
+      __reduce_add_sync(0xffffffffu, unsigned(min(stretches, 1 << 20))) >
+          kChunkCtas)
+    return crossing;
+  // lane l tries a share of crossing + l
+  const int share = int(crossing) + lane;
+  int blocks = 0, lo;
+  for (int s = 0; s < t.sequences; ++s) {
+    const PagedSequence q{0, __shfl_sync(0xffffffffu, line.own.n, s),
+                          __shfl_sync(0xffffffffu, line.own.length, s), false};
+    const int pairs = chunk_pairs(q, units.group);
+    for (int p = 0; p < pairs; ++p)
+      blocks += (chunk_units(q, units.group, units.window, p, lo) + share - 1) /
+                share * kvh;
+  }
+  const unsigned fits = __ballot_sync(0xffffffffu, blocks <= kChunkCtas);
+  if (fits == 0 || __ffs(fits) - 1 > segment)
+    return crossing;
+  const int pad = int(crossing) + __ffs(fits) - 1;
+  line.reset({units.group, units.window, pad});
+  return pad;
+}
+
 // The segment at unit `at` of a range that ends at `end` (warp-wide).
 template <typename Line>
-__device__ bool chunk_segment(const Line& line, int group, int window,
-                              int64_t at, int64_t end, ChunkSegment& g) {
+__device__ bool chunk_segment(const Line& line, int64_t at, int64_t end,
+                              ChunkSegment& g) {
   const int lane = threadIdx.x % 32, kvh = line.t.kv_heads;
+  const ChunkUnits& u = line.units;
+  const int group = u.group, window = u.window;
   int64_t before;
   if (at >= end || !line.find(unit_div(at, kvh), g.seq, g.q, before))
     return false;
@@ -312,7 +369,8 @@ __device__ bool chunk_segment(const Line& line, int group, int window,
     int lo = 0;
     const int64_t mine =
         p0 + lane < pairs
-            ? int64_t(chunk_units(g.q, group, window, p0 + lane, lo)) * kvh
+            ? int64_t(u.rounded(chunk_units(g.q, group, window, p0 + lane,
+                                            lo))) * kvh
             : 0;
     int64_t inc = mine;
 #pragma unroll
@@ -327,9 +385,11 @@ __device__ bool chunk_segment(const Line& line, int group, int window,
       rel -= __shfl_sync(0xffffffffu, inc - mine, l);
       g.pair = p0 + l;
       g.n_units = chunk_units(g.q, group, window, g.pair, g.lo_unit);
-      g.h = int(unit_div(rel, g.n_units));
-      g.u0 = int(rel - int64_t(g.h) * g.n_units);
+      const int stretch = u.rounded(g.n_units);
+      g.h = int(unit_div(rel, stretch));
+      g.u0 = int(rel - int64_t(g.h) * stretch);
       g.count = int(min(int64_t(g.n_units - g.u0), end - at));
+      g.units = g.u0 + g.count == g.n_units ? stretch - g.u0 : g.count;
       return true;
     }
     rel -= __shfl_sync(0xffffffffu, inc, 31);
@@ -382,12 +442,6 @@ __device__ bool weight_segment(const Line& line, int group, int window,
     rel -= __shfl_sync(0xffffffffu, inc, 31);
   }
   return false;
-}
-
-// Units per block for a line of `total` units over `ctas` blocks.
-__device__ __forceinline__ int64_t paged_share(int64_t total, int ctas,
-                                               int least) {
-  return max((total + ctas - 1) / ctas, int64_t(least));
 }
 
 // A stretch that several blocks share: `parts` slots, the first `slot`, then
