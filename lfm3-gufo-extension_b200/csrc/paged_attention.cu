@@ -21,11 +21,10 @@ __device__ __forceinline__ float2 merge(float2& a, float2 b) {
   return make_float2(fa, fb);
 }
 
-// Merges the stretches that several blocks shared. Block b takes record b of
-// the decode kernel (a single token's G heads), then the blocks share out the
-// chunk kernel's records, 32 of a record's 256 rows at a time (only some of its
-// 148 blocks leave one). Slots add up in key order.
-constexpr int kCombineBlocks = kDecodeCtas;
+// Merges the stretches that several blocks shared: the decode kernel's records
+// (a single token's G heads), a head a warp, then the chunk kernel's, 32 of a
+// record's 256 rows a block at a time (only some of its 148 blocks leave one).
+// Slots add up in key order.
 constexpr int kCombineRows = 32;
 
 template <typename T, int DIM>
@@ -35,12 +34,16 @@ __device__ void combine_single(const PagedAttentionArgs& a) {
   const int group = a.heads / a.t.kv_heads;
   const float2* pm = reinterpret_cast<const float2*>(
       a.decode_part + size_t(2 * kDecodeCtas) * group * DIM);
-  const PagedRecord rec = reinterpret_cast<const PagedRecord*>(
-      pm + size_t(2 * kDecodeCtas) * group)[blockIdx.x];
-  if (rec.parts == 0)
-    return;
+  const PagedRecord* records = reinterpret_cast<const PagedRecord*>(
+      pm + size_t(2 * kDecodeCtas) * group);
+  const int warps = blockDim.x / 32;
   // a warp a head, a lane four dimensions
-  for (int j = warp; j < group; j += blockDim.x / 32) {
+  for (int u = blockIdx.x * warps + warp; u < kDecodeCtas * group;
+       u += gridDim.x * warps) {
+    const PagedRecord rec = records[u / group];
+    const int j = u % group;
+    if (rec.parts == 0)
+      continue;
     const float* src = a.decode_part + size_t(j) * DIM + lane % (DIM / 4) * 4;
     const int head = rec.h * group + j;
     float gate = INFINITY;
@@ -260,7 +263,8 @@ cudaError_t launch(PagedAttentionArgs a, uint32_t type, int dim,
   }
   return launch_kernel(dim == 64 ? paged_combine_kernel<T, 64>
                                  : paged_combine_kernel<T, 128>,
-                       dim3(kCombineBlocks), dim3(chunks ? 512 : 128), 0,
+                       dim3(chunks ? kChunkCtas : kDecodeCtas),
+                       dim3(chunks ? 512 : 128), 0,
                        stream, true, a, group <= kDecodeMaxGroup, chunks);
 }
 
