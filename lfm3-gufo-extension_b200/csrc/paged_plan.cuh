@@ -320,7 +320,7 @@ struct ChunkSegment {
 // rounded stretches still fit the blocks is taken, unless crossing shares save
 // more than a second segment costs (its queries, its first copies, its
 // epilogue: about 8 us, `segment` tiles). 512 FP32 rows at depth 8192, 32
-// stretches of 65 to 68 tiles: shares of 17 tiles instead of 15, 91 -> 82 us.
+// stretches of 65 to 68 tiles: shares of 17 tiles instead of 15, 91 -> 88 us.
 __device__ inline int64_t chunk_plan(PagedLine<ChunkUnits>& line,
                                      int segment) {
   const PagedTables& t = line.t;
@@ -466,7 +466,7 @@ __device__ __forceinline__ PagedRecord paged_record(int64_t at, int64_t share,
   return {int(past / share) + 1, slot, q.row0, q.n, pair, h};
 }
 
-// ---- numbers of the softmax ---------------------------------------------------
+// ---- numbers of the softmax ----------------------------------------------
 // Scores are kept in base 2: x = (q k) rsqrt(dim) log2 e.
 constexpr float kLog2e = 1.44269504088896341F;
 constexpr float kLn2 = 0.693147180559945309F;
@@ -498,27 +498,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
-}
-// 2^x on the FMA pipe: n = round(x), 2^(x - n) by a polynomial of degree 4
-// (least squares reweighted to equal relative error, 2.6e-6, two bits below
-// the half step of an fp16), n added to the exponent. Takes x up to 15 (NaN
-// and infinities make the row NaN before); below -125 it is 2^-125.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  x.x = fmaxf(x.x, -125.0F);
-  x.y = fmaxf(x.y, -125.0F);
-  const float2 magic = make_float2(12582912.0F, 12582912.0F);  // 1.5 * 2^23
-  const float2 back = make_float2(-12582912.0F, -12582912.0F);
-  const float2 t = add2(x, magic);
-  const float2 n = add2(t, back);
-  const float2 f = fma2(n, make_float2(-1.0F, -1.0F), x);
-  float2 p = make_float2(0x1.3997d4p-7F, 0x1.3997d4p-7F);
-  p = fma2(p, f, make_float2(0x1.ca1442p-5F, 0x1.ca1442p-5F));
-  p = fma2(p, f, make_float2(0x1.ec06dap-3F, 0x1.ec06dap-3F));
-  p = fma2(p, f, make_float2(0x1.62e0dcp-1F, 0x1.62e0dcp-1F));
-  p = fma2(p, f, make_float2(0x1.ffffe8p-1F, 0x1.ffffe8p-1F));
-  return make_float2(
-      __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 }  // namespace lfm3
