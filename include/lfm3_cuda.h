@@ -293,7 +293,7 @@ int lfm3_sample_host(const float* logits, int rows, int vocab, int ld,
                      const uint32_t* recent_count, const uint64_t* seeds,
                      uint32_t* tokens);
 
-/* ---- paged K/V cache ---------------------------------------------------------
+/* ---- paged K/V cache -------------------------------------------------------
  * No counterpart in the reference, whose sessions own one K/V ring each
  * (engine.cpp:55-77). These operators serve ragged batches of sequences
  * (prompt chunks and single tokens in one call) from one pool of pages per
@@ -310,21 +310,24 @@ int lfm3_sample_host(const float* logits, int rows, int vocab, int ld,
  * table[t / page_rows]. Sequences may share pages (a common prefix) where a
  * call only reads them, lfm3_cuda_paged_attention; lfm3_cuda_paged_heads needs
  * the new rows' pages, _key_weights and _evict all pages unshared (two
- * sequences' sums or moves would meet in one row). Broken tables are not fatal: where starts decrease or
- * pass `rows`, a sequence has more than max_rows rows, a length lies outside
- * 0 .. table_pages * page_rows or a page id that a call needs outside
- * 0 .. pages - 1, nothing outside the buffers is touched, that sequence's
- * results are unspecified and lfm3_cuda_take_device_error() returns 6 after
- * the stream is synchronised. lfm3_paged_check finds the same on the host. */
+ * sequences' sums or moves would meet in one row).
+ *
+ * Broken tables are not fatal: where starts decrease or pass `rows`, a
+ * sequence has more than max_rows rows, a length lies outside 0 .. table_pages
+ * * page_rows or a page id that a call needs outside 0 .. pages - 1, nothing
+ * outside the buffers is touched, that sequence's results are unspecified and
+ * lfm3_cuda_take_device_error() returns 6 after the stream is synchronised (7:
+ * a kernel's bounded wait ran out, and the call's results are unspecified).
+ * lfm3_paged_check finds the same on the host. */
 typedef struct lfm3_paged_cache {
   uint16_t* k; /* F16 [pages][page_rows][kv_heads][dim], 16-byte aligned */
   uint16_t* v;
   const int32_t* table;   /* [sequences][table_stride], page ids */
-  const int32_t* lengths; /* [sequences]: rows held, a call's new rows included */
+  const int32_t* lengths; /* [sequences]: rows held, the new ones included */
   int32_t pages, page_rows; /* page_rows: a multiple of 16 */
   int32_t kv_heads, dim;    /* dim: 64 or 128 */
   int32_t sequences;        /* 0 .. 4096 */
-  int32_t table_pages;      /* entries of a table row in use (most pages of a sequence) */
+  int32_t table_pages;      /* entries of a table row in use */
   int32_t table_stride;     /* >= table_pages */
 } lfm3_paged_cache;
 /* The new rows of a call: rows starts[s] .. starts[s + 1] - 1 of its tensors
@@ -337,7 +340,7 @@ typedef struct lfm3_paged_batch {
   const int32_t* starts;    /* [sequences + 1] */
   const int32_t* positions; /* [rows], or NULL: each row's own number */
   int32_t rows;             /* rows of the tensors */
-  int32_t max_rows;         /* no sequence has more new rows (1: a decode step) */
+  int32_t max_rows; /* no sequence has more new rows (1: a decode step) */
 } lfm3_paged_batch;
 
 /* Checks host copies of the arrays the descriptors point to (k, v and

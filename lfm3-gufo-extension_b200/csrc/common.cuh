@@ -19,7 +19,7 @@ enum DeviceError : unsigned {
   kErrTmemAlloc = 4,
   kErrWaitProbe = 5,  // lfm3_cuda_wait_probe's deliberate wait
   kErrPagedTable = 6,  // a paged call met a broken table
-  kErrPagedWait = 7,
+  kErrPagedWait = 7,   // a paged kernel's bounded wait ran out
 };
 // Defined once in device_error.cu (the library is built with relocatable
 // device code).

@@ -188,6 +188,7 @@ int lfm3_cuda_paged_heads(const lfm3_paged_cache* cache,
     return Invalid("paged heads: q_out is q with another stride");
   CHECK(CheckDevice(cache->k, "paged cache is not on the current device"));
   CHECK(CheckDevice(q, "paged heads: q is not on the current device"));
+  CHECK(CheckDevice(q_out, "paged heads: q_out is not on the current device"));
   lfm3::PagedHeadsArgs a{};
   a.t = Tables(cache, batch);
   a.positions = batch->positions;
@@ -229,6 +230,8 @@ int lfm3_cuda_paged_attention(const lfm3_paged_cache* cache,
   CHECK(CheckRows(q, q_stride, width, "paged attention: q or its stride"));
   CHECK(CheckRows(out, out_stride, width,
                   "paged attention: out or its stride"));
+  if (out == q)
+    return Invalid("paged attention: out may not be q");
   if (gate && (gate_stride < size_t(heads) || gate_stride > size_t(1) << 40))
     return Invalid("paged attention: gate stride");
   const PagedTables t = Tables(cache, batch);
@@ -239,6 +242,7 @@ int lfm3_cuda_paged_attention(const lfm3_paged_cache* cache,
                    "aligned");
   CHECK(CheckDevice(cache->k, "paged cache is not on the current device"));
   CHECK(CheckDevice(q, "paged attention: q is not on the current device"));
+  CHECK(CheckDevice(out, "paged attention: out is not on the current device"));
   if (need)
     CHECK(CheckDevice(
         workspace, "paged attention: workspace is not on the current device"));

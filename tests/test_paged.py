@@ -116,6 +116,8 @@ def test_operator_refusals():
     assert heads(eps=-1.0) == heads(eps=float("inf")) == INVALID
     assert heads(os=264) == INVALID      # in place at another stride
     assert attention(o=None) == attention(os=100) == INVALID
+    assert attention(o=P) == INVALID      # out over q
+    assert b"may not be q" in lfm3.library().lfm3_last_error()
     assert attention(window=-1) == weights(window=-1) == INVALID
     assert attention(gate=P, gs=3) == INVALID
     assert attention(ws=P + 16) == weights(ws=P + 16) == INVALID

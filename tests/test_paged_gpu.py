@@ -245,6 +245,33 @@ def test_sequences_may_share_pages():
     check_attention(p)
 
 
+@pytest.mark.parametrize("page,heads,kv_heads", [(256, 16, 4), (1040, 8, 2),
+                                                 (32, 192, 192),
+                                                 (4096, 384, 3)])
+def test_large_pages_and_many_heads(page, heads, kv_heads):
+    p = Paged([1, 140, 3], [700, 1100, 90], heads, kv_heads, 64, page=page,
+              kind="f16")
+    check_attention(p, gate=True)
+    check_weights(p)
+
+
+def test_outputs_have_to_be_on_the_device():
+    p = Paged([4], [40])
+    host = torch.empty(p.rows, p.heads * p.dim + 8).pin_memory()
+    with pytest.raises(RuntimeError, match="out is not on the current device"):
+        p.attention(out=host)
+    lib, c, b = lfm3.library(), p.cache(), p.batch()
+    f = torch.ones(p.dim // 2, device="cuda")
+    k = torch.zeros(p.rows, p.kv_stride, device="cuda")
+    with pytest.raises(RuntimeError, match="q_out is not on the current"):
+        lfm3.check(lib.lfm3_cuda_paged_heads(
+            ctypes.byref(c), ctypes.byref(b), TYPES["f32"], p.q.data_ptr(),
+            p.q_stride, k.data_ptr(), p.kv_stride, k.data_ptr(), p.kv_stride,
+            host.data_ptr(), host.shape[1], p.heads, None, None, f.data_ptr(),
+            None, 1e-5, p.stream()))
+    check_attention(p)
+
+
 def test_two_calls_at_once():
     """Calls on two streams, each with its own workspace and outputs."""
     one = Paged([1, 300, 1], [4000, 2000, 70], kind="f32", seed=1)
