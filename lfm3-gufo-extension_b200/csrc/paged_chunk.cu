@@ -54,9 +54,10 @@ constexpr int kThreads = 12 * 32;
 constexpr uint32_t kColS = 128, kColO = 256, kColumns = 512;
 constexpr uint32_t kSlab = 128 * 128;  // bytes of [128 rows][64 dims]
 constexpr int kPlanned = 4;            // segments worked out ahead
-// key tiles in the time that a block's second segment takes beyond its tiles
+// key tiles in the time that a segment takes beyond its tiles (2, 3 and 5 for
+// two terms, 4 and 8 for one: up to 5 % and 17 % slower)
 template <int TERMS>
-constexpr int kSegmentUnits = TERMS == 2 ? 3 : 6;
+constexpr int kSegmentUnits = TERMS == 2 ? 4 : 6;
 // exponents (base 2) of a row's largest probability: when the reference
 // moves, and when it has to move again
 constexpr float kTopMoved = 7.0F, kTopLimit = 15.0F;
@@ -197,8 +198,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 11) {
     // ---- the block's segments, then one with count 0
-    PagedLine<ChunkUnits> line(a.t, ChunkUnits{group, a.window, 1});
-    const int64_t share = chunk_plan(line, kSegmentUnits<TERMS>);
+    PagedLine<ChunkUnits> line(
+        a.t, ChunkUnits{group, a.window, 1, kSegmentUnits<TERMS>});
+    const int64_t share = chunk_plan(line);
     if (line.broken && blockIdx.x == 0)
       report_error(kErrPagedTable);
     const int64_t total = line.total * kvh;
@@ -207,6 +209,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     int64_t at = begin;
     for (bool more = true; more && ok; ++planned) {
       more = chunk_segment(line, at, end, g);
+      if (more && g.count == 0) {  // the empty places behind a stretch
+        at += g.units;
+        more = chunk_segment(line, at, end, g);
+      }
       if (!more)
         g.count = g.units = 0;
       g.slot = 2 * blockIdx.x + (at > begin ? 1 : 0);

@@ -17,8 +17,8 @@
 // FP32 queries enter as two fp16 terms and their probabilities too (22 bits);
 // 16-bit queries are exact in one term and the probabilities round to fp16
 // once, which is below their output's own rounding.
-// Measured with the merge: 32 rows over 512 to 32768 keys (597 MB) 110 us,
-// 5.4 TB/s; 8 rows over 85 to 1995 keys 14 us, all of it latency (launches,
+// Measured with the merge: 32 rows over 512 to 32768 keys (597 MB) 104 us,
+// 5.7 TB/s; 8 rows over 85 to 1995 keys 14 us, all of it latency (launches,
 // tables, first copies, merge).
 #include "kernels.cuh"
 #include "paged.cuh"
@@ -110,8 +110,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   grid_dependency_wait();
   allow_dependents();
   const DecodePlan plan = decode_plan(a.t, group, a.window);
-  const DecodeUnits units{group, a.window, plan.pad};
-  const PagedLine line(a.t, units);
+  const DecodeUnits units{group, a.window, plan.pad, plan.extra};
+  PagedLine line(a.t, units);
   if (line.broken && blockIdx.x == 0 && warp == 0)
     report_error(kErrPagedTable);
   const int64_t total = line.total * kvh;
@@ -134,6 +134,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int stretch = units.rounded(n_units);
     const int h = int(unit_div(rel, stretch));
     const int u0 = int(rel - int64_t(h) * stretch);
+    if (u0 >= n_units) {  // the empty places behind a stretch
+      next = at + stretch - u0;
+      continue;
+    }
     const int count = int(min(int64_t(n_units - u0), end - at));
     next = at + (u0 + count == n_units ? stretch - u0 : count);
     // ---- the group's queries are on their way while the page ids come

@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 11) {
     // ---- the block's segments, then one with count 0
-    const PagedLine line(a.t, WeightUnits{group, a.window});
+    PagedLine line(a.t, WeightUnits{group, a.window});
     if (line.broken && blockIdx.x == 0)
       report_error(kErrPagedTable);
     const int64_t total = line.total * kvh;

@@ -57,17 +57,21 @@ __host__ __device__ inline int paged_units(const PagedSequence& q, int window,
 }
 
 // Single tokens share out their line in one of two ways. Equal shares cross
-// from one stretch (a KV head of a sequence) to the next, and a block pays for
+// from one stretch (a KV head of a sequence) to the next. A block pays for
 // each segment (its queries, its first copies, the merge: 3.5 us, the time of
-// kDecodeSegmentUnits units). Rounding every stretch up to a multiple of the
-// share gives a block one segment, at a larger share. The second is taken when
-// it is no slower: short or few sequences (8 rows of 85 to 1995 keys: 9.6 us
-// a launch with crossing shares, 5 us without), while 32 rows of 512 to 32768
-// keys would take 1.7 times as long.
+// kDecodeSegmentUnits units), so a stretch has that many empty places behind
+// it in the line: a block of many short stretches gets fewer units (200
+// sequences of 16 to 8000 keys, 4 KV heads: 271 us without, 157 us with).
+// Rounding every stretch up to a multiple of the share instead gives a block
+// one segment, at a larger share. That is taken when it is no slower: short or
+// few sequences (8 rows of 85 to 1995 keys: 9.6 us a launch with crossing
+// shares, 5 us without), while 32 rows of 512 to 32768 keys would take 1.7
+// times as long.
 constexpr int kDecodeSegmentUnits = 10;
 struct DecodePlan {
   int64_t share;
-  int pad;  // every stretch's units are rounded up to a multiple of this
+  int pad;    // every stretch's units are rounded up to a multiple of this
+  int extra;  // empty places of the line behind each stretch
 };
 
 // Key units of a single-token sequence (0 for every other).
@@ -92,13 +96,16 @@ __device__ inline int chunk_units(const PagedSequence& q, int group,
   return paged_units(q, window, pair * queries,
                      min(q.n, (pair + 1) * queries) - 1, kChunkKeys, lo);
 }
-// Units of every step-th pair from pair `from` on (per KV head), each pair's
-// rounded up to a multiple of `pad`.
+// Places in the line of every step-th pair from pair `from` on (per KV head):
+// its units, rounded up to a multiple of `pad`, and `extra` empty places, the
+// time that a stretch takes beyond its tiles.
 struct ChunkUnits {
   static constexpr bool kMany = true;
-  int group, window, pad;
+  int group, window, pad, extra;
   __device__ int rounded(int units) const {
-    return pad == 1 ? units : (units + pad - 1) / pad * pad;
+    if (units == 0)
+      return 0;
+    return (pad == 1 ? units : (units + pad - 1) / pad * pad) + extra;
   }
   __device__ int64_t operator()(const PagedSequence& q, int from,
                                 int step) const {
@@ -184,16 +191,19 @@ __device__ inline DecodePlan decode_plan(const PagedTables& t, int group,
                     : int64_t((uint32_t(units) + left - 1) / left);
     if (padded <= crossing + kDecodeSegmentUnits)
       return {max(padded, int64_t(kDecodeMinUnits)),
-              int(max(padded, int64_t(kDecodeMinUnits)))};
+              int(max(padded, int64_t(kDecodeMinUnits))), 0};
   }
-  return {crossing, 1};
+  return {max((units + pairs * kDecodeSegmentUnits + kDecodeCtas - 1) /
+                  kDecodeCtas,
+              int64_t(kDecodeMinUnits)),
+          1, kDecodeSegmentUnits};
 }
 
 struct DecodeUnits {
   static constexpr bool kMany = false;
-  int group, window, pad;
+  int group, window, pad, extra;
   __device__ int rounded(int units) const {
-    return (units + pad - 1) / pad * pad;
+    return units == 0 ? 0 : (units + pad - 1) / pad * pad + extra;
   }
   __device__ int64_t operator()(const PagedSequence& q, int, int) const {
     return rounded(decode_units(q, group, window));
@@ -209,7 +219,8 @@ __device__ __forceinline__ int64_t unit_div(int64_t a, int b) {
 // The line of a batch (all members warp-wide); units(sequence, from, step) is
 // every step-th part of a sequence's units from part `from` on. The first 32
 // sequences' entries stay in registers, a lane each: for batches of up to 32
-// the tables are read once. Where a sequence has many parts to sum (kMany), few
+// the tables are read once. Searches go on where the last one ended (1500
+// sequences of 16 to 100 keys: 1087 us from the front, 238 us). Where a sequence has many parts to sum (kMany), few
 // sequences are summed by all lanes together, more a lane each.
 constexpr int kFewSequences = 8;
 template <typename Units>
@@ -220,6 +231,8 @@ struct PagedLine {
   int64_t own_units;
   int64_t total;  // units of the whole batch
   bool broken;    // this lane met a broken sequence
+  int found = 0;  // the 32 sequences that find() ended at, and the units before
+  int64_t found_sum = 0;
 
   __device__ PagedLine(const PagedTables& tables, Units u)
       : t(tables), units(u), own{0, 0, 0, false}, own_units(0), total(0),
@@ -249,7 +262,10 @@ struct PagedLine {
   __device__ void reset(Units u) {
     units = u;
     total = own_units = 0;
-    for (int s = 0; s < t.sequences; ++s) {
+    // (sequences without rows have no units)
+    for (unsigned left = __ballot_sync(0xffffffffu, own.n > 0); left;
+         left &= left - 1) {
+      const int s = __ffs(left) - 1;
       const PagedSequence q{0, __shfl_sync(0xffffffffu, own.n, s),
                             __shfl_sync(0xffffffffu, own.length, s), false};
       const int64_t n = warp_sum64(units(q, threadIdx.x % 32, 32));
@@ -259,13 +275,13 @@ struct PagedLine {
     }
   }
 
-  // The sequence that holds unit `at`, its numbers, and the units before it.
-  // False past the end.
+  // The sequence that holds unit `at` (never before the last one asked for),
+  // its numbers, and the units before it. False past the end.
   __device__ bool find(int64_t at, int& s, PagedSequence& q,
-                       int64_t& before) const {
+                       int64_t& before) {
     const int lane = threadIdx.x % 32;
-    int64_t sum = 0;
-    for (int s0 = 0; s0 < t.sequences; s0 += 32) {
+    int64_t sum = found_sum;
+    for (int s0 = found; s0 < t.sequences; s0 += 32) {
       PagedSequence mine = own;
       int64_t u = own_units;
       if (s0 > 0) {
@@ -292,6 +308,8 @@ struct PagedLine {
         q.length = __shfl_sync(0xffffffffu, mine.length, l);
         q.broken = false;
         before = sum + __shfl_sync(0xffffffffu, inc - u, l);
+        found = s0;
+        found_sum = sum;
         return true;
       }
       sum += __shfl_sync(0xffffffffu, inc, 31);
@@ -315,47 +333,82 @@ struct ChunkSegment {
   int n_units, lo_unit, u0, count, units;
   int slot;
 };
-// The chunks' share and rounding (warp-wide), the same choice as decode_plan's:
-// when there is a block for every stretch, the smallest share with which the
-// rounded stretches still fit the blocks is taken, unless crossing shares save
-// more than a second segment costs (its queries, its first copies, its
-// epilogue: about 8 us, `segment` tiles). 512 FP32 rows at depth 8192, 32
-// stretches of 65 to 68 tiles: shares of 17 tiles instead of 15, 91 -> 88 us.
-__device__ inline int64_t chunk_plan(PagedLine<ChunkUnits>& line,
-                                     int segment) {
+// The chunks' share and places (warp-wide), a similar choice. Equal shares
+// cross stretches, each with `extra` empty places behind it (its queries, its
+// first copies, its epilogue: about 8 us); prompts from position 0 are mostly
+// short stretches (4 of 2000 rows: 285 us without the places, 146 us with).
+// With more stretches than blocks, blocks may take whole ones instead, the same
+// number each: that is no slower when they are about as long (chunks under a
+// window of 256: 50 us crossing, 47 us whole; 24 short chunks at 100 to 300
+// keys, where a block would get one or two: 37 us crossing, 43 us whole), since
+// nothing has to be merged.
+// With fewer, the smallest share with which rounded stretches still fit the
+// blocks is taken, unless crossing shares save more than a second segment
+// costs. 512 FP32 rows at depth 8192, 32 stretches of 65 to 68 tiles: shares
+// of 17 tiles instead of 15, 91 -> 88 us.
+__device__ inline int64_t chunk_plan(PagedLine<ChunkUnits>& line) {
   const PagedTables& t = line.t;
   const ChunkUnits& units = line.units;
-  const int lane = threadIdx.x % 32, kvh = t.kv_heads;
+  const int lane = threadIdx.x % 32, kvh = t.kv_heads, extra = units.extra;
   const int64_t crossing = paged_share(line.total * kvh, kChunkCtas, 1);
-  int stretches = 0;
-  if (lane < t.sequences)
-    stretches = chunk_pairs(line.own, units.group) * kvh;
-  if (t.sequences > 32 || crossing > 1 << 20 ||
-      __reduce_add_sync(0xffffffffu, unsigned(min(stretches, 1 << 20))) >
-          kChunkCtas)
+  if (t.sequences > 32 || crossing > 1 << 20)
     return crossing;
-  // lane l tries a share of crossing + l
-  const int share = int(crossing) + lane;
+  int pairs = 0, some = 0;  // some: those that see a key
+  if (lane < t.sequences) {
+    pairs = chunk_pairs(line.own, units.group);
+    const int idle = max(line.own.n - line.own.length, 0);
+    if (line.own.length > 0)
+      some = pairs - min(pairs, idle / (2 * chunk_queries(units.group)));
+  }
+  const int stretches = __reduce_add_sync(
+      0xffffffffu, unsigned(min(int64_t(some) * kvh, int64_t(1) << 20)));
+  if (stretches > kChunkCtas) {
+    // whole stretches, `each` a block
+    int top = 0, lo;
+    for (unsigned left = __ballot_sync(0xffffffffu, some > 0); left;
+         left &= left - 1) {
+      const int s = __ffs(left) - 1;
+      const PagedSequence q{0, __shfl_sync(0xffffffffu, line.own.n, s),
+                            __shfl_sync(0xffffffffu, line.own.length, s),
+                            false};
+      const int n = __shfl_sync(0xffffffffu, pairs, s);
+      for (int p = lane; p < n; p += 32)
+        top = max(top, chunk_units(q, units.group, units.window, p, lo));
+    }
+    top = __reduce_max_sync(0xffffffffu, unsigned(top));
+    const int each = (stretches + kChunkCtas - 1) / kChunkCtas;
+    if (int64_t(each) * (top + extra) > crossing + extra)
+      return crossing;
+    line.reset({units.group, units.window, top, 0});
+    return int64_t(each) * top;
+  }
+  // lane l tries a share of least + l
+  const int least =
+      int((line.total * kvh - int64_t(stretches) * extra + kChunkCtas - 1) /
+          kChunkCtas);
+  const int share = max(least, 1) + lane;
   int blocks = 0, lo;
-  for (int s = 0; s < t.sequences; ++s) {
+  for (unsigned left = __ballot_sync(0xffffffffu, some > 0); left;
+       left &= left - 1) {
+    const int s = __ffs(left) - 1;
     const PagedSequence q{0, __shfl_sync(0xffffffffu, line.own.n, s),
                           __shfl_sync(0xffffffffu, line.own.length, s), false};
-    const int pairs = chunk_pairs(q, units.group);
-    for (int p = 0; p < pairs; ++p)
+    const int n = __shfl_sync(0xffffffffu, pairs, s);
+    for (int p = 0; p < n; ++p)
       blocks += (chunk_units(q, units.group, units.window, p, lo) + share - 1) /
                 share * kvh;
   }
   const unsigned fits = __ballot_sync(0xffffffffu, blocks <= kChunkCtas);
-  if (fits == 0 || __ffs(fits) - 1 > segment)
+  if (fits == 0 || __ffs(fits) - 1 > extra)
     return crossing;
-  const int pad = int(crossing) + __ffs(fits) - 1;
-  line.reset({units.group, units.window, pad});
+  const int pad = max(least, 1) + __ffs(fits) - 1;
+  line.reset({units.group, units.window, pad, 0});
   return pad;
 }
 
 // The segment at unit `at` of a range that ends at `end` (warp-wide).
 template <typename Line>
-__device__ bool chunk_segment(const Line& line, int64_t at, int64_t end,
+__device__ bool chunk_segment(Line& line, int64_t at, int64_t end,
                               ChunkSegment& g) {
   const int lane = threadIdx.x % 32, kvh = line.t.kv_heads;
   const ChunkUnits& u = line.units;
@@ -388,8 +441,9 @@ __device__ bool chunk_segment(const Line& line, int64_t at, int64_t end,
       const int stretch = u.rounded(g.n_units);
       g.h = int(unit_div(rel, stretch));
       g.u0 = int(rel - int64_t(g.h) * stretch);
-      g.count = int(min(int64_t(g.n_units - g.u0), end - at));
-      g.units = g.u0 + g.count == g.n_units ? stretch - g.u0 : g.count;
+      // (0 where the range begins in the empty places behind a stretch)
+      g.count = int(max(min(int64_t(g.n_units - g.u0), end - at), int64_t(0)));
+      g.units = g.u0 + g.count >= g.n_units ? stretch - g.u0 : g.count;
       return true;
     }
     rel -= __shfl_sync(0xffffffffu, inc, 31);
@@ -407,7 +461,7 @@ struct WeightSegment {
   int slot;
 };
 template <typename Line>
-__device__ bool weight_segment(const Line& line, int group, int window,
+__device__ bool weight_segment(Line& line, int group, int window,
                                int64_t at, int64_t end, WeightSegment& g) {
   const int lane = threadIdx.x % 32, kvh = line.t.kv_heads;
   int64_t before;

@@ -150,6 +150,23 @@ def test_rows_without_keys(kind):
                           kind=kind), gate=True)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [0, 100])
+def test_uneven_lengths(kind, window):
+    """Shares of the work that end between and behind stretches: many short
+    sequences beside a few long ones, single tokens and chunks from row 0."""
+    lengths = [9000] + list(range(1, 60)) * 2 + [4000, 16, 17]
+    check_attention(Paged([1] * len(lengths), lengths, 8, 4, 64, page=32,
+                          kind=kind), window)
+    new = [400, 30, 2, 70, 150]
+    p = Paged(new, [400, 30, 900, 70, 151], 16, 8, 64, page=16, kind=kind)
+    check_attention(p, window, gate=True)
+    check_weights(p, window)
+    new = [1, 65, 1] * 15
+    check_attention(Paged(new, [n + i for i, n in enumerate(new)], 4, 2, 128,
+                          page=16, kind=kind), window)
+
+
 def test_max_rows_is_only_a_bound():
     check_attention(Paged([1, 1, 1], [100, 200, 300], max_rows=500, behind=600))
     check_attention(Paged([40], [100], max_rows=4000, kind="bf16"))
