@@ -220,8 +220,9 @@ __device__ __forceinline__ int64_t unit_div(int64_t a, int b) {
 // every step-th part of a sequence's units from part `from` on. The first 32
 // sequences' entries stay in registers, a lane each: for batches of up to 32
 // the tables are read once. Searches go on where the last one ended (1500
-// sequences of 16 to 100 keys: 1087 us from the front, 238 us). Where a sequence has many parts to sum (kMany), few
-// sequences are summed by all lanes together, more a lane each.
+// sequences of 16 to 100 keys: 1087 us from the front, 238 us). Where a
+// sequence has many parts to sum (kMany), few sequences are summed by all lanes
+// together, more a lane each.
 constexpr int kFewSequences = 8;
 template <typename Units>
 struct PagedLine {
