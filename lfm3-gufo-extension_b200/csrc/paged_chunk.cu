@@ -19,7 +19,10 @@
 // A row's probabilities are 2^(x - m) with a reference m that trails the
 // running maximum: 2^7 for the maximum when m moves, 2^15 at most before it
 // moves again, so it (and with it O in tensor memory) moves rarely and
-// small probabilities stay clear of fp16's subnormals.
+// small probabilities stay clear of fp16's subnormals. Where a step of FP32 is
+// no longer small against these exponents (m past 2^22) a score is rounded to
+// FP32 before m is taken from it, as the maximum was: one fused operation would
+// leave the rounding of the maximum in the exponent, and a probability of 2^64.
 // Masked keys. A key that a row does not see has probability 0, but 0 times a
 // NaN or an infinity in V would still reach the row's sums. In tiles where
 // some row sees less than all keys (the diagonal, a window's edge, the last
@@ -61,6 +64,7 @@ constexpr int kSegmentUnits = TERMS == 2 ? 4 : 6;
 // exponents (base 2) of a row's largest probability: when the reference
 // moves, and when it has to move again
 constexpr float kTopMoved = 7.0F, kTopLimit = 15.0F;
+constexpr float kLargeScore = 4194304.0F;  // its step is 2^-1
 // Tensor-memory sums drop what falls below their last bit, always towards
 // zero: each step of 16 keys and term loses about 2^-24.5 of O. Every so many
 // key tiles O therefore moves to the block's slot, where it is added up with
@@ -673,7 +677,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float top =
             max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3])) * c;
-        const bool move = !(top <= m + kTopLimit);
+        // (the difference is exact where it matters; m + kTopLimit may round)
+        const bool move = !(top <= m) && !(top - m <= kTopLimit);
         if (__any_sync(0xffffffffu, move)) {
           float alpha = 1;
           if (move) {
@@ -698,7 +703,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float shift = m == -INFINITY ? 0.0F : -m;
-        const float2 c2 = make_float2(c, c);
+        const bool large = __any_sync(0xffffffffu, fabsf(shift) > kLargeScore);
+        if (large) {  // columns 0 .. 63 are in v0 and v1, the others still in S
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            v0[i] = __float_as_uint(__fmul_rn(__uint_as_float(v0[i]), c));
+            v1[i] = __float_as_uint(__fmul_rn(__uint_as_float(v1[i]), c));
+          }
+#pragma unroll 1
+          for (int first = 64; first < 128; first += 16) {
+            uint32_t v[16];
+            tc::ld16(ts + first, v);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              v[i] = __float_as_uint(__fmul_rn(__uint_as_float(v[i]), c));
+            tc::st16(ts + first, v);
+          }
+          tc::wait_st();
+        }
+        const float c_now = large ? 1.0F : c;
+        const float2 c2 = make_float2(c_now, c_now);
         const float2 shift2 = make_float2(shift, shift);
         uint32_t ph[16], pl[16];
         const auto compute = [&](const uint32_t(&v)[32]) {

@@ -294,16 +294,20 @@ __global__ void __launch_bounds__(kThreads, 2)
         float pr[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+          // Rounded to FP32 before the maximum is taken from them: past 2^24 one
+          // fused operation would leave the maximum's rounding in the exponent.
+          x[e] = __fmul_rn(x[e], c[nt][e]);
+          x[e + 2] = __fmul_rn(x[e + 2], c[nt][e]);
           float top = fmaxf(x[e], x[e + 2]);
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          top = fmaxf(mrun[nt][e], fmaf(top, c[nt][e], -kTopExponent));
+          top = fmaxf(mrun[nt][e], top - kTopExponent);
           alpha[nt][e] = ex2(mrun[nt][e] - top);
           moved |= top > mrun[nt][e];
           mrun[nt][e] = top;
-          pr[e] = ex2(fmaf(x[e], c[nt][e], -top));
-          pr[e + 2] = ex2(fmaf(x[e + 2], c[nt][e], -top));
+          pr[e] = ex2(x[e] - top);
+          pr[e + 2] = ex2(x[e + 2] - top);
           lrun[nt][e] = lrun[nt][e] * alpha[nt][e] + (pr[e] + pr[e + 2]);
         }
         const SplitPair p0 = split_value(pr[0]), p1 = split_value(pr[1]);

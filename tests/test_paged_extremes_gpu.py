@@ -1,0 +1,104 @@
+"""Paged K/V cache operators on the GPU where numbers or sizes are extreme:
+rows of unlike sizes beside each other, infinite scores, idle rows that hold
+anything, windows past every length, sums that move out of tensor memory many
+times, pools beyond 32-bit offsets. Against the definitions in FP64."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from helpers import lfm3
+from paged import HALF_STEP, TYPES, Paged
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def setup_module(module):
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def broken():
+    torch.cuda.synchronize()
+    return lfm3.library().lfm3_cuda_take_device_error()
+
+
+# Tolerances of single rows. A score is off by at most e = size * (2^-22 +
+# 2 (dim / 16 + 16) 2^-24), size the row's largest sum of |q_d k_d| / sqrt(dim):
+# Q carries 22 bits (F32) or is exact, sums of dim / 16 steps may truncate. The
+# scaled exponential adds 2^-21, the probabilities' rounding 2^-22 (F32) or
+# 2^-11, the sums over keys a step of 2^-23 per 16 keys. Each relative error of
+# a probability enters twice (numerator, denominator), times max |v|, and the
+# output rounds once. Where e is not small, a row whose first score is ahead of
+# the second by 2 e + 40 still has one probability of 1 and others below
+# exp(-40) < 2^-57; rows in between are not compared (but have to be finite).
+def check_rows(p, out, lse, skip=None, window=0):
+    """Every row but those of skip [rows][heads]; returns how many (row, head)
+    pairs were compared, and how many were one-hot."""
+    d, group = p.dim, p.heads // p.kv_heads
+    got = p.host(out)[:, :p.heads * d].reshape(p.rows, p.heads, d)
+    got_lse = p.host(lse)
+    compared = single = 0
+    for s in range(p.seqs):
+        b, length = p.starts[s], p.lengths[s]
+        if not p.new[s]:
+            continue
+        q = p.queries(s)
+        k, v = p.cached(p.k, s, length), p.cached(p.v, s, length)
+        see, top = p.visible(s, window), np.abs(v).max() if length else 0
+        for h in range(p.heads):
+            live = see.any(1)
+            if skip is not None:
+                live &= ~skip[b:b + p.new[s], h]
+            idle = ~see.any(1)
+            assert (got[b:b + p.new[s], h][idle] == 0).all()
+            assert np.isneginf(got_lse[b:b + p.new[s], h][idle]).all()
+            if not live.any():
+                continue
+            kh, vh, qh, sh = k[:, h // group], v[:, h // group], q[live, h], see[live]
+            x = np.where(sh, qh @ kh.T / np.sqrt(d), -np.inf)
+            size = np.where(sh, np.abs(qh) @ np.abs(kh).T / np.sqrt(d), 0).max(1)
+            m = x.max(1, keepdims=True)
+            w = np.exp(x - m)
+            total = w.sum(1, keepdims=True)
+            want, want_lse = w / total @ vh, (m + np.log(total))[:, 0]
+            e = size * (2.0 ** -22 + 2 * (d / 16 + 16) * 2.0 ** -24)
+            x.sort(1)
+            gap = x[:, -1] - x[:, -2] if length > 1 else np.full(len(x), np.inf)
+            small, hot = e < 2.0 ** -6, gap - 2 * e > 40
+            rel = (np.where(hot, 0, np.expm1(np.minimum(e, 1))) + 2.0 ** -21
+                   + (2.0 ** -22 if p.kind == "f32" else 2.0 ** -11)
+                   + (length / 16 + 2) * 2.0 ** -23)
+            y, z = got[b:b + p.new[s], h][live], got_lse[b:b + p.new[s], h][live]
+            assert np.isfinite(y).all() and np.isfinite(z).all()
+            ok = small | hot
+            limit = 2 * rel[:, None] * top + HALF_STEP[p.kind] * np.abs(want) * (
+                1 + 2.0 ** -7) + (2.0 ** -25 if p.kind == "f16" else 0)
+            off = np.abs(y - want)
+            assert (off <= limit)[ok].all(), (s, h, float((off - limit)[ok].max()))
+            assert (np.abs(z - want_lse) <= e + rel + 2.0 ** -22 * np.abs(
+                want_lse))[ok].all()
+            compared += int(ok.sum())
+            single += int((ok & hot).sum())
+    assert broken() == 0
+    return compared, single
+
+
+@pytest.mark.parametrize("kind,power", [("f16", 26), ("f32", 18), ("f32", 21),
+                                        ("f32", 22), ("f32", 24), ("f32", 27),
+                                        ("f32", 60), ("f32", 100), ("bf16", 20),
+                                        ("bf16", 25), ("bf16", 30),
+                                        ("bf16", 110)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scores_of_any_size(kind, power, dim):
+    """Scores past 2^24, where a step of FP32 is 1 or more: rows become one-hot,
+    not infinite."""
+    p = Paged([150, 1, 1, 2], [700, 900, 16, 2], 8, 2, dim, kind=kind, seed=power)
+    if kind == "f16":
+        p.k *= 2.0 ** (power // 2)
+        power -= power // 2
+    p.q *= 2.0 ** power
+    out, lse = p.attention()
+    compared, single = check_rows(p, out, lse)
+    assert compared >= 0.9 * p.rows * p.heads and single > 0.8 * compared
