@@ -15,7 +15,7 @@
 // overwrites its P: tcgen05.mma of one thread run in order.
 // FP32 queries are two fp16 terms (two MMAs for S, two terms of P, which fill
 // the 128 columns of S, two MMAs for O): 22 bits where a 16-bit type has one.
-// Rows are scaled to fp16's range by a power of two first, a batch at a time.
+// Rows are scaled to fp16's range by a power of two each first.
 // A row's probabilities are 2^(x - m) with a reference m that trails the
 // running maximum: 2^7 for the maximum when m moves, 2^15 at most before it
 // moves again, so it (and with it O in tensor memory) moves rarely and
@@ -106,6 +106,27 @@ __device__ __forceinline__ uint32_t clear_not_finite(uint32_t u) {
   if ((u & 0x7C000000u) == 0x7C000000u)
     u &= 0x0000FFFFu;
   return u;
+}
+
+// Maxima of N rows over groups of LANES lanes, N values a lane: the lanes trade
+// halves of their rows (N - 1 shuffles, not N log LANES). Lane `part` of a
+// group gets the maximum of row part / (LANES / N).
+template <int N, int LANES>
+__device__ __forceinline__ float group_max(const float (&v)[N], int part) {
+  if constexpr (LANES == 1) {
+    static_assert(N == 1);
+    return v[0];
+  } else {
+    constexpr int o = LANES / 2, n = N > 1 ? N / 2 : 1;
+    float w[n];
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      const float keep = part & o ? v[N - n + k] : v[k];
+      const float give = part & o ? v[k] : v[N - n + k];
+      w[k] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, o));
+    }
+    return group_max<n, o>(w, part);
+  }
 }
 
 // What a pair of row tiles sees: rows are the sequence's new rows q0 .. qlast.
@@ -504,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the row sees keys oldest .. own
       const int own = live ? range.base + qi : -1;
       const int oldest = a.window > 0 ? max(0, own - a.window + 1) : 0;
-      float c = 0;
+      float c = 1;
       {
         // ---- this warp's 32 rows of Q as fp16 terms
         // (the row tile's warps have read their rows of the last segment)
@@ -516,9 +537,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const size_t offset = row * a.ldq + size_t(head) * DIM;
         const unsigned alive = __ballot_sync(0xffffffffu, live);
         constexpr int kBatch = kRowsAtOnce > 2 ? 32 / kRowsAtOnce : 16;
-        // One power of two brings the batch's rows into fp16's range (none is
-        // needed for fp16 itself): with 29 binades of normal numbers, rows
-        // 2^18 times smaller than the largest still keep their 22 bits.
+        // A power of two of its own brings each row into fp16's range (none is
+        // needed for fp16 itself). The lanes of a row's group hold the scales
+        // of kBatch rows, kSame lanes each.
+        constexpr int kSame = kRowLanes / kBatch;
+        static_assert(kSame * kBatch == kRowLanes);
 #pragma unroll 1
         for (int i0 = 0; i0 < 32; i0 += kBatch * kRowsAtOnce) {
           uint4 raw[kBatch];
@@ -532,21 +555,27 @@ __global__ void __launch_bounds__(kThreads, 1)
               raw[i] = *reinterpret_cast<const uint4*>(
                   static_cast<const T*>(a.q) + at + part * kVec);
           }
-          float scale = 1;
+          float scales = 1;  // of row part / kSame of the lane's group
           if constexpr (!kHalfType) {
-            float top = 0;
+            float top[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
               float v[kVec];
               unpack16(raw[i], v, T{});
+              top[i] = 0;
 #pragma unroll
               for (int k = 0; k < kVec; ++k)
-                top = fmaxf(top, fabsf(v[k]));
+                top[i] = fmaxf(top[i], fabsf(v[k]));
             }
-            scale = row_scale(warp_max(top));
+            scales = row_scale(group_max<kBatch, kRowLanes>(top, part));
+            // this thread's own row: which lane holds its scale
+            const int at = lane - i0;
+            const float mine = __shfl_sync(
+                0xffffffffu, scales,
+                at % kRowsAtOnce * kRowLanes + at / kRowsAtOnce * kSame);
+            if (at >= 0 && at < kBatch * kRowsAtOnce)
+              c = mine;
           }
-          if (lane >= i0 && lane < i0 + kBatch * kRowsAtOnce)
-            c = scale;
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
             const int r = i0 + i * kRowsAtOnce + sub;
@@ -558,6 +587,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               *reinterpret_cast<uint4*>(s.q[x][0] + off) = raw[i];
               continue;
             }
+            const float scale =
+                __shfl_sync(0xffffffffu, scales, lane - part + i * kSame);
             float v[kVec];
             uint32_t hi[kVec / 2], lo[kVec / 2];
             unpack16(raw[i], v, T{});

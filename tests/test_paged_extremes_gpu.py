@@ -102,3 +102,57 @@ def test_scores_of_any_size(kind, power, dim):
     out, lse = p.attention()
     compared, single = check_rows(p, out, lse)
     assert compared >= 0.9 * p.rows * p.heads and single > 0.8 * compared
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (32, 8, 64),
+                                                (3, 1, 128), (16, 1, 64)])
+@pytest.mark.parametrize("power", [18, 24, 32, 40, 100])
+def test_rows_of_unlike_sizes(kind, heads, kv_heads, dim, power):
+    """Heads and queries beside each other whose sizes differ by 2^power: each
+    row keeps its own bits."""
+    p = Paged([150, 1], [400, 200], heads, kv_heads, dim, kind=kind, seed=power)
+    big = torch.zeros(p.rows, heads, dtype=torch.bool, device="cuda")
+    big.view(-1)[2::5] = True
+    q = p.q.view(p.rows, heads, dim)
+    q[big] *= 2.0 ** power
+    out, lse = p.attention()
+    compared, single = check_rows(p, out, lse)
+    # the rows of ordinary size, at least, and most of the others
+    assert compared >= 0.8 * p.rows * heads
+    assert power < 24 or single > 0
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_rows_beside_infinite_queries(kind, dim, value):
+    """A query that is not finite spoils its own rows only, whatever the size of
+    those beside it."""
+    p = Paged([150, 1], [400, 200], 8, 2, dim, kind=kind)
+    bad = np.zeros((p.rows, p.heads), bool)
+    bad.reshape(-1)[2::5] = True
+    q = p.q.view(p.rows, p.heads, dim)
+    q.view(-1, dim)[3::5] *= 2.0 ** 24  # above fp16's largest number
+    q.view(-1, dim)[4::5] *= 2.0 ** -30
+    q.view(-1, dim)[2::5, 7] = value
+    out, lse = p.attention()
+    compared, single = check_rows(p, out, lse, skip=bad)
+    assert compared >= 0.75 * (~bad).sum() and single > 0
+    got = p.host(out)[:, :p.heads * dim].reshape(p.rows, p.heads, dim)
+    assert np.isnan(got[bad]).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("value", [3e4, 1e30, float("inf"), float("nan")])
+def test_idle_rows_may_hold_anything(kind, value):
+    """Rows with negative numbers, and rows that no sequence has, reach no
+    result whatever they hold."""
+    p = Paged([200, 1, 40], [150, 0, 30], 8, 2, 128, kind=kind, before=3,
+              behind=5)
+    idle = list(range(3)) + list(range(p.starts[0], p.starts[0] + 50)) + [
+        int(p.starts[1])] + list(range(p.starts[2], p.starts[2] + 10)) + list(
+        range(p.starts[3], p.rows))
+    p.q[idle] = value
+    out, lse = p.attention()
+    check_rows(p, out, lse)
