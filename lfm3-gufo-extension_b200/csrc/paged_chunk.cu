@@ -139,8 +139,12 @@ struct PairRange {
     base = g.q.length - g.q.n;
     all_hi = base + q0;
     any_hi = base + qlast;
-    all_lo = window > 0 ? max(0, base + qlast - window + 1) : 0;
-    any_lo = window > 0 ? max(0, base + q0 - window + 1) : 0;
+    // (idle rows have negative numbers: compared before the subtraction)
+    const auto oldest = [&](int own) {
+      return window > 0 && own >= window ? own - window + 1 : 0;
+    };
+    all_lo = oldest(base + qlast);
+    any_lo = oldest(base + q0);
   }
   // some row sees less than the whole tile
   __device__ bool edge(int key0) const {
@@ -524,7 +528,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const size_t row = size_t(g.q.row0) + (live ? qi : 0);
       // the row sees keys oldest .. own
       const int own = live ? range.base + qi : -1;
-      const int oldest = a.window > 0 ? max(0, own - a.window + 1) : 0;
+      const int oldest =
+          a.window > 0 && own >= a.window ? own - a.window + 1 : 0;
       float c = 1;
       {
         // ---- this warp's 32 rows of Q as fp16 terms

@@ -156,3 +156,19 @@ def test_idle_rows_may_hold_anything(kind, value):
     p.q[idle] = value
     out, lse = p.attention()
     check_rows(p, out, lse)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 60, 2 ** 30])
+def test_windows_past_every_length(kind, window):
+    """A window that no row fills is no window, in chunks whose first rows have
+    no key, too."""
+    p = Paged([200, 1, 40, 300], [150, 9, 30, 300], 8, 2, 64, kind=kind)
+    out, lse = p.attention(window)
+    want, want_lse = p.attention()
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    check_rows(p, out, lse)
+    start = torch.rand(p.pages, p.page, device="cuda")
+    assert torch.equal(p.key_weights(lse, start.clone(), window),
+                       p.key_weights(lse, start.clone()))
+    assert broken() == 0
