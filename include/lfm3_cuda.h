@@ -370,7 +370,9 @@ int lfm3_cuda_paged_heads(const lfm3_paged_cache* cache,
 /* Causal GQA attention of the new rows over the pages (store their keys and
  * values first): softmax(q k / sqrt(dim)) v over the keys up to the row's own,
  * with window > 0 the last `window` of them; times sigmoid(gate[row][head])
- * where gate is not NULL. A row that sees no key gets 0 and lse -infinity.
+ * where gate is not NULL. A row that sees no key, or none whose score is above
+ * -infinity, gets 0 and lse -infinity. An infinite key gives 16-bit queries the
+ * score of the formula and LFM3_F32 ones (two terms) NaN.
  * q, out [rows][heads][dim] and gate [rows][heads] of `type`; LFM3_F32 keeps
  * Q and the probabilities to 22 bits (two fp16 terms each), 16-bit types
  * round the probabilities to fp16. heads / kv_heads is any whole number up to

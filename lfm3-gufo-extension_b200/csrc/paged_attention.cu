@@ -72,7 +72,8 @@ __device__ void combine_single(const PagedAttentionArgs& a) {
         o.w = o.w * f.x + v[k].w * f.y;
       }
     }
-    const float scale = 1.0F / ml.y / (1 + expf(-gate));
+    // (a sum of 0: no key but scores of -inf, a row like one without keys)
+    const float scale = ml.y == 0 ? 0.0F : 1.0F / ml.y / (1 + expf(-gate));
     T* out = static_cast<T*>(a.out) + size_t(rec.row0) * a.ldo +
              size_t(head) * DIM + lane * 4;
     if (lane < DIM / 4) {

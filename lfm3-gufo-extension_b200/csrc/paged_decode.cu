@@ -303,11 +303,13 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int off = 4; off < 32; off <<= 1)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
           top = fmaxf(mrun[nt][e], top - kTopExponent);
-          alpha[nt][e] = ex2(mrun[nt][e] - top);
+          // (keys whose scores are all -infinity weigh nothing)
+          const float ref = top == -INFINITY ? 0.0F : top;
+          alpha[nt][e] = ex2(mrun[nt][e] - ref);
           moved |= top > mrun[nt][e];
           mrun[nt][e] = top;
-          pr[e] = ex2(x[e] - top);
-          pr[e + 2] = ex2(x[e + 2] - top);
+          pr[e] = ex2(x[e] - ref);
+          pr[e + 2] = ex2(x[e + 2] - ref);
           lrun[nt][e] = lrun[nt][e] * alpha[nt][e] + (pr[e] + pr[e + 2]);
         }
         const SplitPair p0 = split_value(pr[0]), p1 = split_value(pr[1]);
@@ -386,7 +388,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       float l = 0;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        // a warp without keys has maximum -inf and weight 0
+        // a warp without keys, or with none but scores of -inf, has maximum
+        // -inf and weight 0
         const float f = s.wm[w][tid] == -INFINITY ? 0.0F
                                                   : ex2(s.wm[w][tid] - top);
         s.ws[w][tid] = f;
@@ -415,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           pm[j * 2 + d] = d ? s.l[j] : s.m[j];
         continue;
       }
-      y /= s.l[j];
+      y = s.l[j] == 0 ? 0.0F : y / s.l[j];  // 0: no key but scores of -inf
       if (a.gate)
         y /= 1 + expf(-to_float(
                  static_cast<const T*>(a.gate)[size_t(r) * a.ldg + head]));

@@ -172,3 +172,40 @@ def test_windows_past_every_length(kind, window):
     assert torch.equal(p.key_weights(lse, start.clone(), window),
                        p.key_weights(lse, start.clone()))
     assert broken() == 0
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("hidden", [16, 40, 200])
+def test_scores_of_minus_infinity(kind, dim, hidden):
+    """Keys whose score is -infinity (an infinite key, or an FP32 score past
+    the largest number) weigh nothing, in single tokens as in chunks; a row that
+    sees no other key is a row without keys."""
+    p = Paged([1, 40, 1], [200, 240, 200], 8, 2, dim, page=16, kind=kind)
+    if kind == "f16":
+        low, p.q[:, :] = float("-inf"), 1.0
+    else:  # -1e38 * 1000 * dim / sqrt(dim)
+        low, p.q[:, :] = 1000.0, -1e38
+    for s, n in enumerate((hidden, hidden, 200)):
+        for t in range(p.lengths[s]):
+            at = int(p.table[s, t // p.page]), t % p.page
+            p.k[at] = low if t < n else 0.0
+    out, lse = p.attention()
+    got = p.host(out)[:, :8 * dim].reshape(p.rows, 8, dim)
+    got_lse = p.host(lse)
+    for s in range(3):
+        v, see = p.cached(p.v, s, p.lengths[s]), p.visible(s, 0)
+        see[:, :200 if s == 2 else hidden] = False
+        for i in range(p.new[s]):
+            r, count = p.starts[s] + i, see[i].sum()
+            if count == 0:
+                assert (got[r] == 0).all() and np.isneginf(got_lse[r]).all()
+                continue
+            want = v[see[i]].mean(0).repeat(4, 0)  # scores of 0: the mean
+            # probabilities are equal numbers, exact in fp16: the sums' steps
+            # (2^-23 per 16 keys), 1 / l and the output's rounding remain
+            limit = 17 * 2.0 ** -23 * np.abs(v).max() + HALF_STEP[kind] * np.abs(
+                want) * (1 + 2.0 ** -7) + (2.0 ** -25 if kind == "f16" else 0)
+            assert (np.abs(got[r] - want) <= limit).all()
+            assert np.abs(got_lse[r] - np.log(count)).max() <= 8 * 2.0 ** -21
+    assert broken() == 0
