@@ -22,6 +22,7 @@
 // between the two costs what it saves), nor were 64 columns a read (43.6 us).
 // Warps: 8 TMA, 9 tensor memory and MMA, 10 the columns' factors, 11 segments.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.cuh"
 #include "paged.cuh"
@@ -47,6 +48,7 @@ struct __align__(1024) WeightSmem {
   uint8_t k[kKeyStages][2][kTile];
   uint8_t q[kTermStages][kTile];
   float4 factors[2][64];  // of two columns: c, c', -lse, -lse'
+  uint32_t without[2][5];  // columns whose lse is infinite, and whether any is
   uint64_t k_full[kKeyStages], k_empty[kKeyStages];
   uint64_t q_full[kTermStages], q_empty[kTermStages];
   uint64_t f_full[2], f_empty[2];
@@ -95,7 +97,7 @@ __global__ void __launch_bounds__(256)
             __halves2half2(lo[e], lo[e + 1]);
     }
     if (lane == 0) {
-      // a row without keys (lse -inf) adds 2^(0 x - inf)
+      // a row without keys (lse -inf) adds nothing
       const float lse = a.lse[i];
       a.factors[i] = lse == -INFINITY
                          ? make_float2(0, INFINITY)
@@ -326,6 +328,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           s.factors[st][lane * 2 + i] =
               make_float4(f[2 * i].x, f[2 * i + 1].x, -f[2 * i].y,
                           -f[2 * i + 1].y);
+        uint32_t without = 0;  // a lane four columns, eight lanes a word
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          without |= uint32_t(f[i].y == INFINITY) << (lane % 8 * 4 + i);
+        const bool any = __any_sync(0xffffffffu, without);
+        if (any)
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1)
+            without |= __shfl_xor_sync(0xffffffffu, without, o);
+        if (lane % 8 == 0)
+          s.without[st][lane / 8] = without;
+        if (lane == 0)
+          s.without[st][4] = any;
         __syncwarp();
         if (lane == 0)
           mbar_arrive(&s.f_full[st]);
@@ -413,12 +428,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after();
         // Queries q0 .. q0 + nq - 1 of the block; every one sees every key of
         // the tile unless this is an edge. A key is seen from query
-        // key - base on, and by `window` of them.
+        // key - base on, and by `window` of them. Queries without lse are left
+        // out the same way: 2^(x - inf) would be NaN for scores that are.
         const int q0 = b * QB;
         const bool edge = tile1 > base + q0 ||
                           (a.window > 0 &&
                            tile0 <= base + q0 + nq - 1 - a.window) ||
-                          columns % 32 != 0;
+                          columns % 32 != 0 || s.without[half][4];
         const int64_t query = int64_t(key) - base - q0;
         // the key's columns: first .. last - 1
         const int first = int(min(max(query, int64_t(0)), int64_t(nq))) * group;
@@ -427,41 +443,50 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ? int(min(max(query + a.window, int64_t(0)), int64_t(nq))) *
                       group
                 : columns;
+        const auto add_up = [&](auto some_hidden) {
 #pragma unroll 1
-        for (int c0 = 0; c0 < columns; c0 += 32) {
-          uint32_t v[32];
-          tc::ld32(td + c0, v);
-          float4 f[16];
+          for (int c0 = 0; c0 < columns; c0 += 32) {
+            uint32_t v[32];
+            tc::ld32(td + c0, v);
+            float4 f[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            f[i] = s.factors[half][c0 / 2 + i];
-          tc::wait_ld();
-          const unsigned a0 = max(first - c0, 0), a1 = max(last - c0, 0);
-          // columns a0 .. a1 - 1 of the 32 see the key
-          const uint32_t seen =
-              a1 <= a0 || a0 > 31
-                  ? 0u
-                  : (0xffffffffu >> (32 - (min(a1, 32u) - a0))) << a0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 p = fma2(make_float2(__uint_as_float(v[2 * i]),
-                                        __uint_as_float(v[2 * i + 1])),
-                            make_float2(f[i].x, f[i].y),
-                            make_float2(f[i].z, f[i].w));
-            if (edge) {
-              if (!(seen >> (2 * i) & 1))
-                p.x = -INFINITY;
-              if (!(seen >> (2 * i + 1) & 1))
-                p.y = -INFINITY;
+            for (int i = 0; i < 16; ++i)
+              f[i] = s.factors[half][c0 / 2 + i];
+            uint32_t seen = 0xffffffffu;
+            if constexpr (some_hidden) {
+              // columns a0 .. a1 - 1 of the 32 see the key
+              const unsigned a0 = max(first - c0, 0), a1 = max(last - c0, 0);
+              seen = a1 <= a0 || a0 > 31
+                         ? 0u
+                         : (0xffffffffu >> (32 - (min(a1, 32u) - a0))) << a0;
+              seen &= ~s.without[half][c0 / 32];
             }
-            p.x = ex2(p.x);
-            p.y = ex2(p.y);
-            if (i % 2)
-              sum1 = add2(sum1, p);
-            else
-              sum0 = add2(sum0, p);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float2 p = fma2(make_float2(__uint_as_float(v[2 * i]),
+                                          __uint_as_float(v[2 * i + 1])),
+                              make_float2(f[i].x, f[i].y),
+                              make_float2(f[i].z, f[i].w));
+              if constexpr (some_hidden) {
+                if (!(seen >> (2 * i) & 1))
+                  p.x = -INFINITY;
+                if (!(seen >> (2 * i + 1) & 1))
+                  p.y = -INFINITY;
+              }
+              p.x = ex2(p.x);
+              p.y = ex2(p.y);
+              if (i % 2)
+                sum1 = add2(sum1, p);
+              else
+                sum0 = add2(sum0, p);
+            }
           }
-        }
+        };
+        if (edge)
+          add_up(std::true_type{});
+        else
+          add_up(std::false_type{});
         tc::fence_before();
         __syncwarp();
         if (lane == 0) {

@@ -209,3 +209,45 @@ def test_scores_of_minus_infinity(kind, dim, hidden):
             assert (np.abs(got[r] - want) <= limit).all()
             assert np.abs(got_lse[r] - np.log(count)).max() <= 8 * 2.0 ** -21
     assert broken() == 0
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), 1.0])
+def test_weights_of_rows_without_lse(kind, value):
+    """A query whose lse is -infinity adds nothing, whatever it and the keys
+    hold: among others, a whole column block of them, single tokens."""
+    p = Paged([150, 1, 1, 70], [900, 300, 290, 600], 8, 2, 128, kind=kind)
+    lse = p.attention()[1]
+    off = torch.zeros(p.rows, 8, dtype=torch.bool, device="cuda")
+    off.view(-1)[5::7] = True
+    off[32:64] = True            # queries 32 .. 63: a column block
+    off[p.starts[2]] = True
+    q = p.q.view(p.rows, 8, 128)
+    q[off] = value
+    lse[off] = float("-inf")
+    # a key that only such rows see: sequence 3's last
+    off[p.rows - 1] = True
+    lse[p.rows - 1] = float("-inf")
+    last = int(p.table[3, 599 // p.page]), 599 % p.page
+    p.k[last] = float("-inf") if value == 1.0 else value
+    start = torch.rand(p.pages, p.page, device="cuda") + 0.5
+    got = p.host(p.key_weights(lse, start.clone()))
+    z, want = p.host(lse), p.host(start)
+    p.q = torch.where(off[:, :, None], torch.zeros_like(q), q).view(p.rows, -1)
+    p.k[last] = 0.0
+    scale = 1.0
+    for s in range(p.seqs):
+        i = np.arange(p.lengths[s])
+        place = p.table[s, i // p.page], i % p.page
+        had = want[place]
+        had[p.lengths[s] - p.new[s]:] = 0
+        want[place] = had + p.expect_weights(s, z)
+        scale = max(scale, p.expect_attention(s)[2])
+    assert got[last] == 0
+    # a probability carries its score's error and the exponential's, and sums
+    # of n * heads of them round by a step of 2^-24 each
+    rel = (scale * (2.0 ** -22 + 2 * (128 / 16 + 16) * 2.0 ** -24) + 2.0 ** -20
+           + (150 * 8 + 8) * 2.0 ** -24 + 2.0 ** -23 * np.abs(
+               z[np.isfinite(z)]).max())
+    assert (np.abs(got - want) <= rel * np.abs(want) + 1e-30).all()
+    assert broken() == 0
