@@ -199,9 +199,6 @@ struct PagedAttentionArgs {
   alignas(64) CUtensorMap kmap;
   alignas(64) CUtensorMap vmap;
   int box_rows;
-  // the chunk kernel was launched behind the decode kernel of the same call,
-  // which waited for the work before it
-  bool behind_decode;
   PagedTables t;
   const void* q;
   const void* gate;

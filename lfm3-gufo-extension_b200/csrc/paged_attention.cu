@@ -252,7 +252,6 @@ cudaError_t launch(PagedAttentionArgs a, uint32_t type, int dim,
   }
   const bool chunks = !paged_single(a.t.max_rows, group);
   if (chunks) {
-    a.behind_decode = group <= kDecodeMaxGroup;
     // the largest box that never crosses a page
     a.box_rows = std::min(a.t.page_rows & -a.t.page_rows, kChunkKeys);
     if ((e = encode_pool_map(&a.kmap, a.t.k, pool, a.t.kv_heads, dim,

@@ -193,13 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == 9)
     tc::alloc(&s.tmem, kColumns);
-  // Behind the decode kernel this grid may start once every block of that one
-  // is past its own wait, so all that came before it has ended. What an SM has
-  // cached from before that may be stale: the fence drops it.
-  if (a.behind_decode)
-    __threadfence();
-  else
-    grid_dependency_wait();
+  grid_dependency_wait();
   allow_dependents();
   tc::fence_before();
   __syncthreads();
@@ -948,8 +942,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   }
-  if (a.behind_decode)
-    grid_dependency_wait();  // this grid ends after the decode kernel's
   tc::fence_before();
   __syncthreads();
   if (warp == 9) {
