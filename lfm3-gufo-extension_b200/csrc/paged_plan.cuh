@@ -361,8 +361,8 @@ __device__ inline int64_t chunk_plan(PagedLine<ChunkUnits>& line) {
     if (line.own.length > 0)
       some = pairs - min(pairs, idle / (2 * chunk_queries(units.group)));
   }
-  const int stretches = __reduce_add_sync(
-      0xffffffffu, unsigned(min(int64_t(some) * kvh, int64_t(1) << 20)));
+  // (64 bits: the shares below hold every stretch, however many there are)
+  const int64_t stretches = warp_sum64(int64_t(some) * kvh);
   if (stretches > kChunkCtas) {
     // whole stretches, `each` a block
     int top = 0, lo;
@@ -377,16 +377,15 @@ __device__ inline int64_t chunk_plan(PagedLine<ChunkUnits>& line) {
         top = max(top, chunk_units(q, units.group, units.window, p, lo));
     }
     top = __reduce_max_sync(0xffffffffu, unsigned(top));
-    const int each = (stretches + kChunkCtas - 1) / kChunkCtas;
-    if (int64_t(each) * (top + extra) > crossing + extra)
+    const int64_t each = (stretches + kChunkCtas - 1) / kChunkCtas;
+    if (each * (top + extra) > crossing + extra)
       return crossing;
     line.reset({units.group, units.window, top, 0});
-    return int64_t(each) * top;
+    return each * top;
   }
   // lane l tries a share of least + l
   const int least =
-      int((line.total * kvh - int64_t(stretches) * extra + kChunkCtas - 1) /
-          kChunkCtas);
+      int((line.total * kvh - stretches * extra + kChunkCtas - 1) / kChunkCtas);
   const int share = max(least, 1) + lane;
   int blocks = 0, lo;
   for (unsigned left = __ballot_sync(0xffffffffu, some > 0); left;
