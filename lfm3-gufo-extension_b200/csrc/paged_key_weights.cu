@@ -126,6 +126,14 @@ __device__ __forceinline__ void add_weight(const PagedKeyWeightsArgs& a,
 struct WeightRecord {
   int parts, slot, seq, pair;
 };
+// Bytes of the slots of sums and the records behind them, and of the factors:
+// every part of the workspace begins on a 256-byte boundary.
+constexpr size_t kPartBytes =
+    (size_t(2 * kWeightCtas) * kWeightKeys * sizeof(float) +
+     kWeightCtas * sizeof(WeightRecord) + 255) / 256 * 256;
+constexpr size_t factor_bytes(size_t values) {
+  return (values * sizeof(float2) + 255) / 256 * 256;
+}
 
 template <int DIM, int TERMS>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -533,14 +541,11 @@ cudaError_t launch(PagedKeyWeightsArgs a, cudaStream_t stream) {
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   const int kvh = a.t.kv_heads, group = a.heads / kvh;
   const size_t values = size_t(a.t.rows) * a.heads;
-  // (the parts stay 256-byte aligned)
-  a.part = static_cast<float*>(a.workspace);
-  a.factors = reinterpret_cast<float2*>(
-      a.part + size_t(2 * kWeightCtas) * kWeightKeys +
-      kWeightCtas * sizeof(WeightRecord) / 4);
-  a.terms = reinterpret_cast<__half*>(
-      reinterpret_cast<char*>(a.factors) +
-      (values * sizeof(float2) + 255) / 256 * 256);
+  char* space = static_cast<char*>(a.workspace);
+  a.part = reinterpret_cast<float*>(space);
+  a.factors = reinterpret_cast<float2*>(space + kPartBytes);
+  a.terms =
+      reinterpret_cast<__half*>(space + kPartBytes + factor_bytes(values));
   a.box_rows = std::min(a.t.page_rows & -a.t.page_rows, 128);
   cudaError_t e;
   if ((e = encode_pool_map(&a.kmap, a.t.k, a.t.pages * a.t.page_rows, kvh, DIM,
@@ -577,9 +582,7 @@ cudaError_t launch(const PagedKeyWeightsArgs& a, int dim,
 
 size_t paged_key_weights_workspace(const PagedTables& t, int dim, int heads) {
   const size_t values = size_t(t.rows) * heads;
-  return size_t(2 * kWeightCtas) * kWeightKeys * 4 +
-         kWeightCtas * sizeof(WeightRecord) +
-         (values * sizeof(float2) + 255) / 256 * 256 + values * dim * 2 * 2;
+  return kPartBytes + factor_bytes(values) + values * dim * 2 * sizeof(__half);
 }
 
 cudaError_t launch_paged_key_weights(const PagedKeyWeightsArgs& a,
