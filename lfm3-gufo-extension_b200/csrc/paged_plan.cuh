@@ -25,7 +25,6 @@ constexpr int kDecodeMaxGroup = 16;   // more heads per KV head: chunk kernel
 // Chunks: tiles of 128 keys against pairs of 128-row tiles.
 constexpr int kChunkKeys = 128;
 constexpr int kChunkCtas = 148;       // one per SM
-constexpr int kChunkMinUnits = 1;
 constexpr int kChunkRows = 128;       // (query, head of the group) rows, M
 
 __host__ __device__ inline bool paged_single(int n, int group) {
@@ -187,7 +186,7 @@ __device__ inline DecodePlan decode_plan(const PagedTables& t, int group,
   if (pairs < kDecodeCtas) {
     const uint32_t left = uint32_t(kDecodeCtas - pairs);
     const int64_t padded =
-        units >> 31 ? units / left
+        units >> 31 ? (units + left - 1) / left
                     : int64_t((uint32_t(units) + left - 1) / left);
     if (padded <= crossing + kDecodeSegmentUnits)
       return {max(padded, int64_t(kDecodeMinUnits)),
