@@ -3,6 +3,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdio>
+#include <initializer_list>
 #include <memory>
 #include <new>
 
@@ -31,6 +32,14 @@ int Status(cudaError_t e) {
 bool Aligned16(const void* p) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 }
+// Kernels read and write arrays an element at a time at least: each has to be
+// aligned to its elements (a misaligned access would end the context). NULL is.
+bool Aligned(size_t bytes, std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays)
+    if (reinterpret_cast<uintptr_t>(p) % bytes)
+      return false;
+  return true;
+}
 
 // The descriptors' own numbers and pointers. dim and kv_heads first: the
 // other operators answer UNSUPPORTED for shapes, whatever the pointers are.
@@ -56,6 +65,8 @@ int CheckCache(const lfm3_paged_cache* c) {
     return Invalid("paged cache: NULL array");
   if (!Aligned16(c->k) || !Aligned16(c->v))
     return Invalid("paged cache: k and v must be 16-byte aligned");
+  if (!Aligned(4, {c->table, c->lengths}))
+    return Invalid("paged cache: table or lengths are not aligned");
   return LFM3_OK;
 }
 int CheckBatch(const lfm3_paged_batch* b) {
@@ -63,6 +74,8 @@ int CheckBatch(const lfm3_paged_batch* b) {
     return Invalid("paged batch descriptor is NULL");
   if (!b->starts || b->rows < 0 || b->max_rows < 0)
     return Invalid("paged batch: starts, rows and max_rows");
+  if (!Aligned(4, {b->starts, b->positions}))
+    return Invalid("paged batch: starts or positions are not aligned");
   return LFM3_OK;
 }
 int CheckType(uint32_t type) {
@@ -175,6 +188,8 @@ int lfm3_cuda_paged_heads(const lfm3_paged_cache* cache,
   CHECK(CheckHeads(heads, cache));
   if (!frequencies || !(eps >= 0) || !std::isfinite(eps))
     return Invalid("paged heads: frequencies and eps");
+  if (!Aligned(4, {q_norm, k_norm, frequencies, factors}))
+    return Invalid("paged heads: norms, frequencies or factors are not aligned");
   if (batch->rows == 0 || cache->sequences == 0 || batch->max_rows == 0)
     return LFM3_OK;
   const size_t width = size_t(heads) * cache->dim;
@@ -234,6 +249,8 @@ int lfm3_cuda_paged_attention(const lfm3_paged_cache* cache,
     return Invalid("paged attention: out may not be q");
   if (gate && (gate_stride < size_t(heads) || gate_stride > size_t(1) << 40))
     return Invalid("paged attention: gate stride");
+  if (!Aligned(type == LFM3_F32 ? 4 : 2, {gate}) || !Aligned(4, {lse}))
+    return Invalid("paged attention: gate or lse are not aligned");
   const PagedTables t = Tables(cache, batch);
   const size_t need = lfm3::paged_attention_workspace(t, cache->dim, heads);
   if (workspace_bytes < need || (need && !workspace) ||
@@ -283,6 +300,8 @@ int lfm3_cuda_paged_key_weights(const lfm3_paged_cache* cache,
                   "paged key weights: q or its stride"));
   if (!lse || !weights)
     return Invalid("paged key weights: lse and weights");
+  if (!Aligned(4, {lse, weights}))
+    return Invalid("paged key weights: lse or weights are not aligned");
   const PagedTables t = Tables(cache, batch);
   const size_t need = lfm3::paged_key_weights_workspace(t, cache->dim, heads);
   if (workspace_bytes < need || (need && !workspace) ||
@@ -312,6 +331,8 @@ int lfm3_cuda_paged_evict(const lfm3_paged_cache* cache,
   CHECK(CheckCache(cache));
   if (!out_table || !out_lengths || !weights || !kept)
     return Invalid("paged evict: NULL array");
+  if (!Aligned(4, {out_table, out_lengths, weights, kept}))
+    return Invalid("paged evict: an array is not aligned");
   if (keep < 1 || recent < 0 || recent > keep)
     return Invalid("paged evict: keep must be positive, recent 0..keep");
   if (int64_t(cache->table_pages) * cache->page_rows < keep)

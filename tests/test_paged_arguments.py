@@ -1,0 +1,77 @@
+"""Paged K/V cache operators: arguments that no kernel may get, refused on the
+host before any CUDA call (no GPU)."""
+import ctypes
+
+import pytest
+
+from helpers import abi, lfm3
+
+P = 0x10000  # never dereferenced
+INVALID = -1
+
+
+def cache(**over):
+    d = dict(k=P, v=P, table=P, lengths=P, pages=10, page_rows=16, kv_heads=2,
+             dim=64, sequences=2, table_pages=4, table_stride=4)
+    return abi.PagedCache(**{**d, **over})
+
+
+def batch(**over):
+    return abi.PagedBatch(**{**dict(starts=P, positions=None, rows=4, max_rows=4),
+                             **over})
+
+
+def heads(c=None, b=None, kind=0, q=P, qs=256, k=4 * P, ks=128, v=5 * P, vs=128,
+          o=2 * P, os=256, qn=P, kn=P, freq=P, fac=None):
+    return lfm3.library().lfm3_cuda_paged_heads(
+        ctypes.byref(c or cache()), ctypes.byref(b or batch()), kind, q, qs, k,
+        ks, v, vs, o, os, 4, qn, kn, freq, fac, 1e-5, None)
+
+
+def attention(c=None, b=None, kind=0, q=P, qs=256, gate=None, o=2 * P, os=256,
+              lse=None):
+    return lfm3.library().lfm3_cuda_paged_attention(
+        ctypes.byref(c or cache()), ctypes.byref(b or batch()), kind, q, qs, gate,
+        4, o, os, lse, 4, 0, P, 1 << 40, None)
+
+
+def weights(c=None, b=None, lse=P, w=P):
+    return lfm3.library().lfm3_cuda_paged_key_weights(
+        ctypes.byref(c or cache()), ctypes.byref(b or batch()), 0, P, 256, lse, w,
+        4, 0, P, 1 << 40, None)
+
+
+def evict(c=None, out_table=P, out_lengths=P, w=P, kept=P):
+    return lfm3.library().lfm3_cuda_paged_evict(
+        ctypes.byref(c or cache()), out_table, out_lengths, w, kept, 8, 2, None)
+
+
+def refused(code, text):
+    message = lfm3.library().lfm3_last_error()
+    return code == INVALID and text in message
+
+
+@pytest.mark.parametrize("name", ["table", "lengths"])
+def test_misaligned_tables(name):
+    c = cache(**{name: P + 2})
+    for call in (heads, attention, weights, evict):
+        assert refused(call(c), b"table or lengths are not aligned")
+
+
+@pytest.mark.parametrize("name", ["starts", "positions"])
+def test_misaligned_batch(name):
+    b = batch(**{name: P + 1})
+    for call in (heads, attention, weights):
+        assert refused(call(b=b), b"starts or positions are not aligned")
+
+
+def test_misaligned_arrays():
+    for name in ("qn", "kn", "freq", "fac"):
+        assert refused(heads(**{name: P + 2}), b"are not aligned")
+    assert refused(attention(lse=P + 2), b"gate or lse")
+    assert refused(attention(gate=P + 2), b"gate or lse")        # FP32
+    assert refused(attention(kind=1, gate=P + 1), b"gate or lse")
+    for name in ("lse", "w"):
+        assert refused(weights(**{name: P + 2}), b"lse or weights")
+    for name in ("out_table", "out_lengths", "w", "kept"):
+        assert refused(evict(**{name: P + 3}), b"an array is not aligned")
