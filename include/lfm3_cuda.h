@@ -298,12 +298,15 @@ int lfm3_sample_host(const float* logits, int rows, int vocab, int ld,
  * (engine.cpp:55-77). These operators serve ragged batches of sequences
  * (prompt chunks and single tokens in one call) from one pool of pages per
  * attention layer, and shrink sequences that have grown too long. All take
- * device pointers except the descriptors themselves, allocate nothing, keep
- * nothing between calls and only queue work on `stream`, so they can be
- * captured into a CUDA graph: a replay reads starts, positions, table and
- * lengths afresh, everything else (the descriptors' numbers too) is as
- * captured. Calls that may overlap on the GPU need workspaces of their own,
- * two captured graphs that may be replayed at once included.
+ * pointers that the current device reaches, except the descriptors themselves:
+ * its own or managed memory, for arrays other than pools, queries, their
+ * outputs, eviction's weights and workspaces pinned host memory, too; others
+ * are refused. All allocate nothing, keep nothing between calls and only queue
+ * work on `stream`, so they can be captured into a CUDA graph: a replay reads
+ * starts, positions, table and lengths afresh, everything else (the
+ * descriptors' numbers too) is as captured. Calls that may overlap on the GPU
+ * need workspaces of their own, two captured graphs that may be replayed at
+ * once included.
  *
  * A sequence's rows (one cached key and value each) are numbered from 0 in
  * the order of its tokens; row t lies in row t % page_rows of page

@@ -96,20 +96,46 @@ int CheckRows(const void* p, size_t stride, size_t width, const char* what) {
     return Invalid(what);
   return LFM3_OK;
 }
-// The caller's memory has to be of the current device, where the kernels run.
-int CheckDevice(const void* p, const char* what) {
-  int device = 0;
-  cudaPointerAttributes at{};
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess)
-    e = cudaPointerGetAttributes(&at, p);
-  if (e != cudaSuccess)
-    return Status(e);
-  if ((at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) ||
-      (at.type == cudaMemoryTypeDevice && at.device != device))
-    return Invalid(what);
-  return LFM3_OK;
-}
+// The caller's memory has to be of the current device, where the kernels run:
+// pools, queries, their outputs and workspaces in its own or managed memory, the
+// other arrays (`small`) may be pinned host memory, too. Pageable memory and another
+// device's would end the context.
+struct Memory {
+  int device = -1;
+  int status = LFM3_OK;
+  int check(const void* p, bool small, const char* what) {
+    if (status != LFM3_OK || !p)
+      return status;
+    cudaPointerAttributes at{};
+    cudaError_t e = device < 0 ? cudaGetDevice(&device) : cudaSuccess;
+    if (e == cudaSuccess)
+      e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess)
+      return status = Status(e);
+    if (at.type == cudaMemoryTypeManaged ||
+        (at.type == cudaMemoryTypeDevice && at.device == device) ||
+        (at.type == cudaMemoryTypeHost && small))
+      return LFM3_OK;
+    return status = Invalid(what);
+  }
+  int check(const lfm3_paged_cache* c) {
+    constexpr const char* what = "paged cache is not on the current device";
+    check(c->k, false, what);
+    check(c->v, false, what);
+    check(c->table, true, what);
+    return check(c->lengths, true, what);
+  }
+  int check(const lfm3_paged_batch* b) {
+    constexpr const char* what = "paged batch is not on the current device";
+    check(b->starts, true, what);
+    return check(b->positions, true, what);
+  }
+  int check(std::initializer_list<const void*> arrays, const char* what) {
+    for (const void* p : arrays)
+      check(p, true, what);
+    return status;
+  }
+};
 
 PagedTables Tables(const lfm3_paged_cache* c, const lfm3_paged_batch* b) {
   PagedTables t{};
@@ -201,9 +227,17 @@ int lfm3_cuda_paged_heads(const lfm3_paged_cache* cache,
                   "paged heads: q_out or its stride"));
   if (q_out == q && q_out_stride != q_stride)
     return Invalid("paged heads: q_out is q with another stride");
-  CHECK(CheckDevice(cache->k, "paged cache is not on the current device"));
-  CHECK(CheckDevice(q, "paged heads: q is not on the current device"));
-  CHECK(CheckDevice(q_out, "paged heads: q_out is not on the current device"));
+  Memory memory;
+  CHECK(memory.check(cache));
+  CHECK(memory.check(batch));
+  CHECK(memory.check(q, false, "paged heads: q is not on the current device"));
+  CHECK(memory.check(q_out, false,
+                     "paged heads: q_out is not on the current device"));
+  CHECK(memory.check({k, v}, "paged heads: k or v is not on the current "
+                             "device"));
+  CHECK(memory.check({q_norm, k_norm, frequencies, factors},
+                     "paged heads: norms, frequencies or factors are not on "
+                     "the current device"));
   lfm3::PagedHeadsArgs a{};
   a.t = Tables(cache, batch);
   a.positions = batch->positions;
@@ -257,12 +291,18 @@ int lfm3_cuda_paged_attention(const lfm3_paged_cache* cache,
       reinterpret_cast<uintptr_t>(workspace) % 256)
     return Invalid("paged attention: workspace too small or not 256-byte "
                    "aligned");
-  CHECK(CheckDevice(cache->k, "paged cache is not on the current device"));
-  CHECK(CheckDevice(q, "paged attention: q is not on the current device"));
-  CHECK(CheckDevice(out, "paged attention: out is not on the current device"));
+  Memory memory;
+  CHECK(memory.check(cache));
+  CHECK(memory.check(batch));
+  CHECK(memory.check(q, false,
+                     "paged attention: q is not on the current device"));
+  CHECK(memory.check(out, false,
+                     "paged attention: out is not on the current device"));
   if (need)
-    CHECK(CheckDevice(
-        workspace, "paged attention: workspace is not on the current device"));
+    CHECK(memory.check(workspace, false, "paged attention: workspace is not on "
+                                         "the current device"));
+  CHECK(memory.check({gate, lse}, "paged attention: gate or lse is not on the "
+                                  "current device"));
   lfm3::PagedAttentionArgs a{};
   a.t = t;
   a.q = q, a.gate = gate, a.out = out, a.lse = lse;
@@ -308,11 +348,16 @@ int lfm3_cuda_paged_key_weights(const lfm3_paged_cache* cache,
       reinterpret_cast<uintptr_t>(workspace) % 256)
     return Invalid("paged key weights: workspace too small or not 256-byte "
                    "aligned");
-  CHECK(CheckDevice(cache->k, "paged cache is not on the current device"));
-  CHECK(CheckDevice(q, "paged key weights: q is not on the current device"));
+  Memory memory;
+  CHECK(memory.check(cache));
+  CHECK(memory.check(batch));
+  CHECK(memory.check(q, false,
+                     "paged key weights: q is not on the current device"));
   if (need)
-    CHECK(CheckDevice(workspace, "paged key weights: workspace is not on the "
-                                 "current device"));
+    CHECK(memory.check(workspace, false, "paged key weights: workspace is not "
+                                         "on the current device"));
+  CHECK(memory.check({lse, weights}, "paged key weights: lse or weights are "
+                                     "not on the current device"));
   lfm3::PagedKeyWeightsArgs a{};
   a.t = t;
   a.q = q, a.lse = lse, a.weights = weights;
@@ -339,9 +384,12 @@ int lfm3_cuda_paged_evict(const lfm3_paged_cache* cache,
     return Invalid("paged evict: a sequence's pages hold fewer than keep rows");
   if (cache->sequences == 0)
     return LFM3_OK;
-  CHECK(CheckDevice(cache->k, "paged cache is not on the current device"));
-  CHECK(CheckDevice(weights, "paged evict: weights are not on the current "
-                             "device"));
+  Memory memory;
+  CHECK(memory.check(cache));
+  CHECK(memory.check(weights, false, "paged evict: weights are not on the "
+                                     "current device"));
+  CHECK(memory.check({out_table, out_lengths, kept},
+                     "paged evict: an array is not on the current device"));
   lfm3::PagedEvictArgs a{};
   a.t = Tables(cache, nullptr);
   a.out_table = out_table;
