@@ -357,10 +357,11 @@ int lfm3_paged_check(const lfm3_paged_cache* cache,
  * arithmetic of lfm3_cuda_prompt_heads over a ragged batch; a NULL norm
  * weight leaves that norm out) with the keys and values stored in their
  * pages, in one pass. q [rows][heads][dim], k and v [rows][kv_heads][dim] and
- * q_out (may be q) are of `type` (LFM3_F32, LFM3_F16 or LFM3_BF16), rows
- * `*_stride` elements apart (a multiple of 8; 16-byte aligned); arithmetic in
- * FP32, angles position * frequencies[i] / factors[i] in FP64 (factors may be
- * NULL), one rounding to q_out's type and to F16. */
+ * q_out (q itself, or rows that overlap none of q's, k's and v's) are of
+ * `type` (LFM3_F32, LFM3_F16 or LFM3_BF16), rows `*_stride` elements apart (a
+ * multiple of 8; 16-byte aligned); arithmetic in FP32, angles position *
+ * frequencies[i] / factors[i] in FP64 (factors may be NULL), one rounding to
+ * q_out's type and to F16. */
 int lfm3_cuda_paged_heads(const lfm3_paged_cache* cache,
                           const lfm3_paged_batch* batch, uint32_t type,
                           const void* q, size_t q_stride, const void* k,

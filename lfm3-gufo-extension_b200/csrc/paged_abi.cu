@@ -1,5 +1,6 @@
 // extern "C" entry points of the paged K/V cache operators: argument checks
 // (before any CUDA call), then one launcher each.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdio>
@@ -95,6 +96,37 @@ int CheckRows(const void* p, size_t stride, size_t width, const char* what) {
       stride > size_t(1) << 40)
     return Invalid(what);
   return LFM3_OK;
+}
+// `rows` rows of `width` elements, `stride` elements apart.
+struct Rows {
+  const void* p;
+  size_t stride, width;
+};
+// Whether a row of a and a row of b have a byte in common (columns of one
+// buffer do not, though their ranges overlap).
+bool Overlap(const Rows& a, const Rows& b, int rows, uint32_t type) {
+  using Wide = __int128;
+  const size_t size = type == LFM3_F32 ? 4 : 2;
+  const Wide a0 = reinterpret_cast<uintptr_t>(a.p), aw = a.width * size;
+  const Wide b0 = reinterpret_cast<uintptr_t>(b.p), bw = b.width * size;
+  const Wide as = Wide(a.stride) * size, bs = Wide(b.stride) * size;
+  if (a0 + (rows - 1) * as + aw <= b0 || b0 + (rows - 1) * bs + bw <= a0)
+    return false;
+  // in the order of addresses: the row that ends first meets no later one
+  for (Wide i = 0, j = 0; i < rows && j < rows;) {
+    const Wide x = a0 + i * as, y = b0 + j * bs;
+    if (x + aw > y && y + bw > x)
+      return true;
+    // rows that end before the other's begin, all at once
+    if (x + aw <= y)
+      i += std::max<Wide>((y - x - aw) / as, 1);
+    else
+      j += std::max<Wide>((x - y - bw) / bs, 1);
+    // equal strides: what holds for one pair of neighbours holds for all
+    if (as == bs && i > 0 && j > 0)
+      return false;
+  }
+  return false;
 }
 // The caller's memory has to be of the current device, where the kernels run:
 // pools, queries, their outputs and workspaces in its own or managed memory, the
@@ -227,6 +259,11 @@ int lfm3_cuda_paged_heads(const lfm3_paged_cache* cache,
                   "paged heads: q_out or its stride"));
   if (q_out == q && q_out_stride != q_stride)
     return Invalid("paged heads: q_out is q with another stride");
+  const Rows to{q_out, q_out_stride, width};
+  if ((q_out != q && Overlap(to, {q, q_stride, width}, batch->rows, type)) ||
+      Overlap(to, {k, k_stride, kv}, batch->rows, type) ||
+      Overlap(to, {v, v_stride, kv}, batch->rows, type))
+    return Invalid("paged heads: q_out overlaps q, k or v");
   Memory memory;
   CHECK(memory.check(cache));
   CHECK(memory.check(batch));
@@ -281,6 +318,8 @@ int lfm3_cuda_paged_attention(const lfm3_paged_cache* cache,
                   "paged attention: out or its stride"));
   if (out == q)
     return Invalid("paged attention: out may not be q");
+  if (Overlap({out, out_stride, width}, {q, q_stride, width}, batch->rows, type))
+    return Invalid("paged attention: out overlaps q");
   if (gate && (gate_stride < size_t(heads) || gate_stride > size_t(1) << 40))
     return Invalid("paged attention: gate stride");
   if (!Aligned(type == LFM3_F32 ? 4 : 2, {gate}) || !Aligned(4, {lse}))

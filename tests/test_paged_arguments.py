@@ -1,6 +1,7 @@
 """Paged K/V cache operators: arguments that no kernel may get, refused on the
 host before any CUDA call (no GPU)."""
 import ctypes
+import random
 
 import pytest
 
@@ -75,3 +76,47 @@ def test_misaligned_arrays():
         assert refused(weights(**{name: P + 2}), b"lse or weights")
     for name in ("out_table", "out_lengths", "w", "kept"):
         assert refused(evict(**{name: P + 3}), b"an array is not aligned")
+
+
+def overlap(a, sa, wa, b, sb, wb, rows):
+    """Whether row i of a and row j of b share a byte, for some i and j < rows."""
+    return any(a + i * sa < b + j * sb + wb and b + j * sb < a + i * sa + wa
+               for i in range(rows) for j in range(rows))
+
+
+def test_overlapping_rows_are_refused():
+    """Exactly the calls whose rows overlap: columns of one buffer are fine."""
+    rng = random.Random(0)
+    base, text = 1 << 32, b"overlaps"
+    seen = [0, 0]
+    for _ in range(3000):
+        rows = rng.choice([1, 2, 3, 7, 12])
+        kind, size = rng.choice([(0, 4), (1, 2), (30, 2)])
+        width = 4 * 64 * size
+        sq = rng.choice([256, 264, 512, 768, 1024])
+        so = rng.choice([sq, sq, 256, 328, 600, 2048])
+        q = base + 16 * rng.randint(0, 40)
+        o = q + 16 * rng.choice([rng.randint(-400, 400), rng.randint(-9000, 9000)])
+        if o == q:
+            continue
+        want = overlap(q, sq * size, width, o, so * size, width, rows)
+        seen[want] += 1
+        b = batch(rows=rows)
+        far = dict(k=1 << 40, v=1 << 41)
+        for call in (lambda: attention(b=b, kind=kind, q=q, qs=sq, o=o, os=so),
+                     lambda: heads(b=b, kind=kind, q=q, qs=sq, o=o, os=so, **far)):
+            code = call()
+            # calls that are not refused end at the first CUDA call here, or at
+            # the pointers that are not the device's
+            assert (code == INVALID and
+                    text in lfm3.library().lfm3_last_error()) == want, (
+                        rows, kind, sq, so, o - q)
+            assert code != 0
+    assert min(seen) > 300
+    # keys and values, and a fused buffer [q k v] worked on in place
+    q, row = base, (256 + 128 + 128)
+    fused = dict(q=q, qs=row, k=q + 1024, ks=row, v=q + 1536, vs=row, os=row)
+    assert not refused(heads(o=q, **fused), text)
+    assert refused(heads(o=q + 1024, **fused), text)
+    assert refused(heads(o=q + 512, **fused), text)
+    assert refused(heads(**{**fused, "q": 1 << 40, "o": q + 1280}), text)
