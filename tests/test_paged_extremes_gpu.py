@@ -251,3 +251,116 @@ def test_weights_of_rows_without_lse(kind, value):
                z[np.isfinite(z)]).max())
     assert (np.abs(got - want) <= rel * np.abs(want) + 1e-30).all()
     assert broken() == 0
+
+
+# ---- sums that move out of tensor memory -----------------------------------------
+def spikes(p, s):
+    """Every 600 keys of sequence s one whose score is 6.5 or 12.5 above the
+    others', in turn: rows move their reference, and what they have summed up
+    before still counts."""
+    b, e = p.starts[s], p.starts[s + 1]
+    p.q[b:e].view(e - b, -1)[:, :p.heads * p.dim:p.dim] = 8.0
+    at = torch.from_numpy(p.table[s].astype(np.int64)).cuda()
+    pages = -(-p.lengths[s] // p.page)
+    p.k[at[:pages], :, :, 0] = 0.0
+    for j, t in enumerate(range(300, p.lengths[s], 600)):
+        p.k[int(p.table[s, t // p.page]), t % p.page, :, 0] = (
+            (6.5, 12.5)[j % 2] * p.dim ** 0.5 / 8)
+
+
+# In the 2-norm. FP32 rows: 64 additions in tensor memory (4 tiles of 8 steps and
+# two terms) drop half a step of 2^-23 each, of a sum that grows from 0: 1.9e-6;
+# the scores' sums shrink by 8 such halves in 16 steps, 5e-7 of scores of size
+# 1.3 to 2; Q's and P's roundings of 2^-23 are independent and a tenth of that.
+# 4e-6 bounds their sum. Spikes: scores of 12.5 instead of 2, 8e-6. A flush that
+# is lost or counted twice changes the sums by a tile's share or more: 1e-2.
+def norm_off(p, s, rows, out, lse):
+    """The rows' error in the 2-norm against FP64, and the lse's largest."""
+    d, group = p.dim, p.heads // p.kv_heads
+    k, v = p.cached(p.k, s, p.lengths[s]), p.cached(p.v, s, p.lengths[s])
+    base = p.lengths[s] - p.new[s]
+    q = p.queries(s)
+    square = off = worst = 0.0
+    for i in rows:
+        own = base + i
+        for h in range(p.heads):
+            x = k[:own + 1, h // group] @ q[i, h] / np.sqrt(d)
+            m = x.max()
+            w = np.exp(x - m)
+            want = w @ v[:own + 1, h // group] / w.sum()
+            got = p.host(out[p.starts[s] + i, h * d:(h + 1) * d])
+            off += float(((got - want) ** 2).sum())
+            square += float((want ** 2).sum())
+            z = float(lse[p.starts[s] + i, h])
+            worst = max(worst, abs(z - (m + np.log(w.sum()))) / max(1, abs(z)))
+    return (off / square) ** 0.5, worst
+
+
+@pytest.mark.parametrize("moving", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim,n,length", [
+    (16, 4, 128, 512, 8704), (32, 8, 64, 512, 8300), (8, 8, 64, 2300, 5000),
+    (4, 4, 128, 256, 12000)])
+def test_sums_moved_many_times(moving, heads, kv_heads, dim, n, length):
+    """FP32 rows over segments of 9 to 40 key tiles: their sums leave tensor
+    memory every 4 tiles and are added up, with the reference unmoved or moved
+    in between."""
+    p = Paged([n], [length], heads, kv_heads, dim, page=128)
+    if moving:
+        spikes(p, 0)
+    out, lse = p.attention()
+    off, worst = norm_off(p, 0, (0, 1, n // 3, n // 2 + 7, n - 1), out, lse)
+    assert off <= (8e-6 if moving else 4e-6) and worst <= 4e-6
+    assert broken() == 0
+
+
+# ---- offsets past 32 bits -------------------------------------------------------
+def test_pools_past_32_bit_offsets():
+    """Pools of 5 GB whose held pages lie at both ends: element and byte offsets
+    pass 2^32."""
+    p = Paged([60, 1, 0], [300, 700, 0], 8, 2, 128, page=64, kind="bf16",
+              extra_pages=5)
+    small, pages = p.pages, 5 * 2 ** 30 // (64 * 2 * 128 * 2)
+    for name in ("k", "v"):
+        x = torch.zeros(pages, 64, 2, 128, dtype=torch.float16, device="cuda")
+        x[:8] = getattr(p, name)[:8]
+        x[pages - (small - 8):] = getattr(p, name)[8:]
+        setattr(p, name, x)
+    assert p.k.numel() > 2 ** 31 and p.k.numel() * 2 > 2 ** 32
+    p.table[p.table >= 8] += pages - small
+    p.pages, p.dtable = pages, torch.from_numpy(p.table).cuda()
+    out, lse = p.attention()
+    check_rows(p, out, lse)
+    start = torch.rand(pages, 64, device="cuda")
+    got = p.host(p.key_weights(lse, start.clone()))
+    want, z = p.host(start), p.host(lse)
+    for s in range(2):
+        i = np.arange(p.lengths[s])
+        place = p.table[s, i // 64], i % 64
+        had = want[place]
+        had[p.lengths[s] - p.new[s]:] = 0
+        want[place] = had + p.expect_weights(s, z)
+    assert (np.abs(got - want) <= 1e-4 * np.abs(want)).all()
+    # heads: the keys as they are (no norm, angles of 0) into the same places
+    new = torch.randn(p.rows, 256, device="cuda").to(p.q.dtype)
+    q, zero = p.q.clone(), torch.zeros(64, device="cuda")
+    c, b = p.cache(), p.batch()
+    lfm3.check(lfm3.library().lfm3_cuda_paged_heads(
+        ctypes.byref(c), ctypes.byref(b), TYPES["bf16"], q.data_ptr(),
+        p.q_stride, new.data_ptr(), 256, new.data_ptr(), 256, q.data_ptr(),
+        p.q_stride, 8, None, None, zero.data_ptr(), None, 0.0, p.stream()))
+    held = [p.cached(p.k, s, p.lengths[s]) for s in range(2)]
+    for s in range(2):
+        x = p.host(new[p.starts[s]:p.starts[s + 1]].half()).reshape(-1, 2, 128)
+        assert np.array_equal(held[s][p.lengths[s] - p.new[s]:], x)
+    # eviction in place
+    weights = torch.rand(pages, 64, device="cuda")
+    kept = torch.full((3, 100), -1, dtype=torch.int32, device="cuda")
+    lfm3.check(lfm3.library().lfm3_cuda_paged_evict(
+        ctypes.byref(c), p.dtable.data_ptr(), p.dlengths.data_ptr(),
+        weights.data_ptr(), kept.data_ptr(), 100, 10, p.stream()))
+    for s in range(2):
+        rows = kept[s].cpu().numpy()
+        assert (np.diff(rows) > 0).all() and rows[-10:].min() == p.lengths[s] - 10
+        assert np.array_equal(p.cached(p.k, s, 100), held[s][rows])
+    assert p.dlengths.tolist() == [100, 100, 0]
+    assert broken() == 0
