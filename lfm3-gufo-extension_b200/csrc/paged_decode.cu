@@ -17,9 +17,9 @@
 // FP32 queries enter as two fp16 terms and their probabilities too (22 bits);
 // 16-bit queries are exact in one term and the probabilities round to fp16
 // once, which is below their output's own rounding.
-// Measured with the merge: 32 rows over 512 to 32768 keys (597 MB) 104 us,
-// 5.7 TB/s; 8 rows over 85 to 1995 keys 14 us, all of it latency (launches,
-// tables, first copies, merge).
+// Measured with the merge: 32 rows over 512 to 32768 keys (597 MB) 103 us,
+// 5.8 TB/s (FP32 rows 105 us); 8 rows over 85 to 1995 keys 15 us, all of it
+// latency (launches, tables, first copies, merge).
 #include "kernels.cuh"
 #include "paged.cuh"
 #include "paged_plan.cuh"

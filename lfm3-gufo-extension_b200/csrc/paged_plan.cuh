@@ -60,11 +60,12 @@ __host__ __device__ inline int paged_units(const PagedSequence& q, int window,
 // each segment (its queries, its first copies, the merge: 3.5 us, the time of
 // kDecodeSegmentUnits units), so a stretch has that many empty places behind
 // it in the line: a block of many short stretches gets fewer units (200
-// sequences of 16 to 8000 keys, 4 KV heads: 271 us without, 157 us with).
+// sequences of 16 to 8000 keys, 4 KV heads: 233 us without, 131 us with).
 // Rounding every stretch up to a multiple of the share instead gives a block
 // one segment, at a larger share. That is taken when it is no slower: short or
-// few sequences (8 rows of 85 to 1995 keys: 9.6 us a launch with crossing
-// shares, 5 us without), while 32 rows of 512 to 32768 keys would take 1.7
+// few sequences (8 rows of 100 keys 9.0 us padded, 10.9 us crossing, with the
+// merge; of 1000 keys 11.5 and 13.0 us; where both are near, padded ones are up
+// to 2 % slower), while 32 rows of 512 to 32768 keys would take 1.7
 // times as long.
 constexpr int kDecodeSegmentUnits = 10;
 struct DecodePlan {
@@ -336,16 +337,20 @@ struct ChunkSegment {
 // The chunks' share and places (warp-wide), a similar choice. Equal shares
 // cross stretches, each with `extra` empty places behind it (its queries, its
 // first copies, its epilogue: about 8 us); prompts from position 0 are mostly
-// short stretches (4 of 2000 rows: 285 us without the places, 146 us with).
+// short stretches (4 of 2000 rows: 279 us without the places, 144 us with).
 // With more stretches than blocks, blocks may take whole ones instead, the same
 // number each: that is no slower when they are about as long (chunks under a
-// window of 256: 50 us crossing, 47 us whole; 24 short chunks at 100 to 300
-// keys, where a block would get one or two: 37 us crossing, 43 us whole), since
-// nothing has to be merged.
+// window of 256: 53 us crossing, 50.5 us whole), since nothing has to be merged.
+// (24 chunks of 30 to 40 rows at 100 to 300 keys show the estimate's limits: 38 us
+// whole, as it says, 35 us crossing.)
 // With fewer, the smallest share with which rounded stretches still fit the
 // blocks is taken, unless crossing shares save more than a second segment
-// costs. 512 FP32 rows at depth 8192, 32 stretches of 65 to 68 tiles: shares
-// of 17 tiles instead of 15, 91 -> 88 us.
+// costs. That is worth 15 % where stretches are few and short (1024 f16 rows at
+// depth 1000 48 us padded, 56 us crossing) and costs up to 4 % where they are
+// long (512 FP32 rows at depth 8192, 32 stretches of 65 to 68 tiles, shares of 17
+// tiles instead of 15: 91 us padded, 88 us crossing) and 17 % for 200 f16 rows
+// from position 0 (23 and 19 us); over 72 batches of 1 to 4 chunks the two are
+// within 1 %.
 __device__ inline int64_t chunk_plan(PagedLine<ChunkUnits>& line) {
   const PagedTables& t = line.t;
   const ChunkUnits& units = line.units;
