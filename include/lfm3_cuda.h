@@ -343,7 +343,8 @@ typedef struct lfm3_paged_batch {
   const int32_t* starts;    /* [sequences + 1] */
   const int32_t* positions; /* [rows], or NULL: each row's own number */
   int32_t rows;             /* rows of the tensors */
-  int32_t max_rows; /* no sequence has more new rows (1: a decode step) */
+  int32_t max_rows; /* no sequence has more new rows (1: a decode step; 0: the
+                       call does nothing) */
 } lfm3_paged_batch;
 
 /* Checks host copies of the arrays the descriptors point to (k, v and
