@@ -75,8 +75,8 @@ int CheckBatch(const lfm3_paged_batch* b) {
     return Invalid("paged batch descriptor is NULL");
   if (!b->starts || b->rows < 0 || b->max_rows < 0)
     return Invalid("paged batch: starts, rows and max_rows");
-  if (!Aligned(4, {b->starts, b->positions}))
-    return Invalid("paged batch: starts or positions are not aligned");
+  if (!Aligned(4, {b->starts}))
+    return Invalid("paged batch: starts are not aligned");
   return LFM3_OK;
 }
 int CheckType(uint32_t type) {
@@ -166,17 +166,18 @@ struct Memory {
       return LFM3_OK;
     return status = Invalid(what);
   }
-  int check(const lfm3_paged_cache* c) {
+  // (what an operator does not read is not looked at: key weights need no
+  // values, heads alone read positions)
+  int check(const lfm3_paged_cache* c, bool values = true) {
     constexpr const char* what = "paged cache is not on the current device";
     check(c->k, false, what);
-    check(c->v, false, what);
+    if (values)
+      check(c->v, false, what);
     check(c->table, true, what);
     return check(c->lengths, true, what);
   }
   int check(const lfm3_paged_batch* b) {
-    constexpr const char* what = "paged batch is not on the current device";
-    check(b->starts, true, what);
-    return check(b->positions, true, what);
+    return check(b->starts, true, "paged batch is not on the current device");
   }
   int check(std::initializer_list<const void*> arrays, const char* what) {
     for (const void* p : arrays)
@@ -262,8 +263,9 @@ int lfm3_cuda_paged_heads(const lfm3_paged_cache* cache,
   CHECK(CheckHeads(heads, cache));
   if (!frequencies || !(eps >= 0) || !std::isfinite(eps))
     return Invalid("paged heads: frequencies and eps");
-  if (!Aligned(4, {q_norm, k_norm, frequencies, factors}))
-    return Invalid("paged heads: norms, frequencies or factors are not aligned");
+  if (!Aligned(4, {batch->positions, q_norm, k_norm, frequencies, factors}))
+    return Invalid("paged heads: positions, norms, frequencies or factors are "
+                   "not aligned");
   if (batch->rows == 0 || cache->sequences == 0 || batch->max_rows == 0)
     return LFM3_OK;
   const size_t width = size_t(heads) * cache->dim;
@@ -288,9 +290,9 @@ int lfm3_cuda_paged_heads(const lfm3_paged_cache* cache,
                      "paged heads: q_out is not on the current device"));
   CHECK(memory.check({k, v}, "paged heads: k or v is not on the current "
                              "device"));
-  CHECK(memory.check({q_norm, k_norm, frequencies, factors},
-                     "paged heads: norms, frequencies or factors are not on "
-                     "the current device"));
+  CHECK(memory.check({batch->positions, q_norm, k_norm, frequencies, factors},
+                     "paged heads: positions, norms, frequencies or factors are "
+                     "not on the current device"));
   lfm3::PagedHeadsArgs a{};
   a.t = Tables(cache, batch);
   a.positions = batch->positions;
@@ -404,7 +406,7 @@ int lfm3_cuda_paged_key_weights(const lfm3_paged_cache* cache,
     return Invalid("paged key weights: workspace too small or not 256-byte "
                    "aligned");
   Memory memory;
-  CHECK(memory.check(cache));
+  CHECK(memory.check(cache, false));
   CHECK(memory.check(batch));
   CHECK(memory.check(q, false,
                      "paged key weights: q is not on the current device"));

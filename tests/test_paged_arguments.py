@@ -59,11 +59,13 @@ def test_misaligned_tables(name):
         assert refused(call(c), b"table or lengths are not aligned")
 
 
-@pytest.mark.parametrize("name", ["starts", "positions"])
-def test_misaligned_batch(name):
-    b = batch(**{name: P + 1})
+def test_misaligned_batch():
     for call in (heads, attention, weights):
-        assert refused(call(b=b), b"starts or positions are not aligned")
+        assert refused(call(b=batch(starts=P + 1)), b"starts are not aligned")
+    # heads alone read positions
+    assert refused(heads(b=batch(positions=P + 1)), b"are not aligned")
+    for call in (attention, weights):
+        assert not refused(call(b=batch(positions=P + 1)), b"aligned")
 
 
 def test_misaligned_arrays():

@@ -60,11 +60,11 @@ class Call:
             c, a["out_table"], a["out_lengths"], a["weights"], a["kept"], 30, 2, s)
 
 
-BATCH = ["k", "v", "table", "lengths", "starts", "positions"]
+BATCH = ["k", "table", "lengths", "starts"]
 ARRAYS = {
-    "heads": BATCH + ["q", "out", "knew", "vnew", "q_norm", "k_norm", "freq",
-                      "factors"],
-    "attention": BATCH + ["q", "out", "gate", "lse", "space"],
+    "heads": BATCH + ["v", "positions", "q", "out", "knew", "vnew", "q_norm",
+                      "k_norm", "freq", "factors"],
+    "attention": BATCH + ["v", "q", "out", "gate", "lse", "space"],
     "weights": BATCH + ["q", "lse", "weights", "space"],
     "evict": ["k", "v", "table", "lengths", "out_table", "out_lengths", "weights",
               "kept"],
@@ -113,3 +113,12 @@ def test_small_arrays_may_be_pinned(op):
         results.append([call.own[name].cpu().clone() for name in names])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("op,name", [("attention", "positions"),
+                                     ("weights", "positions"), ("weights", "v")])
+def test_what_an_operator_does_not_read_may_be_anything(op, name):
+    call = Call()
+    assert call(op, **{name: 0x10000}) == 0
+    torch.cuda.synchronize()
+    assert lfm3.library().lfm3_cuda_take_device_error() == 0
