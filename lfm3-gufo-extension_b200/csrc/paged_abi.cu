@@ -129,9 +129,9 @@ bool Overlap(const Rows& a, const Rows& b, int rows, uint32_t type) {
   return false;
 }
 // The caller's memory has to be of the current device, where the kernels run:
-// pools, queries, their outputs and workspaces in its own or managed memory, the
-// other arrays (`small`) may be pinned host memory, too. Pageable memory and another
-// device's would end the context.
+// pools, queries, their outputs and workspaces in its own or managed memory,
+// the other arrays (`small`) may be pinned host memory, too. Pageable memory
+// and another device's would end the context.
 // The driver is asked for three attributes at once: 34 ns an array, where
 // cudaPointerGetAttributes takes 58 (a call has up to 14).
 struct Memory {
@@ -291,8 +291,8 @@ int lfm3_cuda_paged_heads(const lfm3_paged_cache* cache,
   CHECK(memory.check({k, v}, "paged heads: k or v is not on the current "
                              "device"));
   CHECK(memory.check({batch->positions, q_norm, k_norm, frequencies, factors},
-                     "paged heads: positions, norms, frequencies or factors are "
-                     "not on the current device"));
+                     "paged heads: positions, norms, frequencies or factors "
+                     "are not on the current device"));
   lfm3::PagedHeadsArgs a{};
   a.t = Tables(cache, batch);
   a.positions = batch->positions;
@@ -336,7 +336,8 @@ int lfm3_cuda_paged_attention(const lfm3_paged_cache* cache,
                   "paged attention: out or its stride"));
   if (out == q)
     return Invalid("paged attention: out may not be q");
-  if (Overlap({out, out_stride, width}, {q, q_stride, width}, batch->rows, type))
+  if (Overlap({out, out_stride, width}, {q, q_stride, width}, batch->rows,
+              type))
     return Invalid("paged attention: out overlaps q");
   if (gate && (gate_stride < size_t(heads) || gate_stride > size_t(1) << 40))
     return Invalid("paged attention: gate stride");

@@ -35,14 +35,14 @@
 // 32 rows, a row at a time over the lanes), 8 TMA, 9 tensor memory and (one
 // thread) every MMA, 10 the clearing, 11 works out the segments ahead of the
 // others. Every wait is bounded.
-// Two chunks of 2048 bf16 rows at depth 16384 (504 GFLOP): 525 to 547 us, 0.92 to
-// 0.96 PFLOP/s, the clock falling under the power limit when repeated. Neither
-// the tensor cores nor the special function units are full (each busy for 42 %
-// of two chunks of 1000 rows at depth 5000): the chain of S, softmax and P V of
-// two row tiles is. A polynomial on the FMA pipe for an eighth of the
-// exponentials gained 1 % and cost bits, so there is none. 512 FP32 rows at depth
-// 8192 (two terms, 71 GFLOP as such): 90 us with the merge, of which 60 us are
-// key tiles, the rest the single-token kernel before it, the plan, the queries'
+// Two chunks of 2048 bf16 rows at depth 16384 (504 GFLOP): 525 to 547 us, 0.92
+// to 0.96 PFLOP/s, the clock falling under the power limit. Neither the tensor
+// cores nor the special function units are full (each busy for 42 % of two
+// chunks of 1000 rows at depth 5000): the chain of S, softmax and P V of two
+// row tiles is. A polynomial on the FMA pipe for an eighth of the exponentials
+// gained 1 % and cost bits, so there is none. 512 FP32 rows at depth 8192 (two
+// terms, 71 GFLOP as such): 90 us with the merge, of which 60 us are key tiles,
+// the rest the single-token kernel before it, the plan, the queries'
 // conversion, O's moves and the merge.
 #include <type_traits>
 
@@ -72,8 +72,8 @@ constexpr float kLargeScore = 4194304.0F;  // its step is 2^-1
 // key tiles O therefore moves to the block's slot, where it is added up with
 // rounding. FP32 rows: every 4 tiles (512 rows at depth 8192: 5.3e-6 off in
 // the 2-norm and 83 us without, 1.6e-6 and 94 us with; every 2 tiles 1.0e-6
-// and 101 us; repeated). fp16 rows: before the loss nears their own half step. bf16 rows
-// would take more than 2^20 keys a block to notice, and never do.
+// and 101 us; repeated). fp16 rows: before the loss nears their own half step.
+// bf16 rows would take more than 2^20 keys a block to notice, and never do.
 template <typename T>
 constexpr int kFlushTiles = 1 << 30;
 template <>

@@ -294,8 +294,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         float pr[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          // Rounded to FP32 before the maximum is taken from them: past 2^24 one
-          // fused operation would leave the maximum's rounding in the exponent.
+          // Rounded to FP32 before the maximum is taken from them: past 2^24
+          // one fused operation would leave the maximum's rounding in the
+          // exponent.
           x[e] = __fmul_rn(x[e], c[nt][e]);
           x[e + 2] = __fmul_rn(x[e + 2], c[nt][e]);
           float top = fmaxf(x[e], x[e + 2]);

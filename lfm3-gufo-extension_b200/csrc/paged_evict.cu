@@ -15,11 +15,12 @@
 //         writes alone: rows in batches, a batch's reads all done before its
 //         writes, and no write touches what a later batch reads (kept[j] >=
 //         j), so the next batch is read before the barrier, too.
-// One sequence of 32000 rows of 4 heads of 128, 8192 kept: 27 us into other pages,
-// most of it the selection's latency (three passes over eight SMs); 48 us in
-// place, where a block moves a single 16-byte column, half a sector, so that all
-// SMs have one. 24 sequences of 900 to 9000 rows, 2000 kept: 55 us either way
-// (26 us are the bytes: the weights once, each kept row once each way).
+// One sequence of 32000 rows of 4 heads of 128, 8192 kept: 27 us into other
+// pages, most of it the selection's latency (three passes over eight SMs); 48
+// us in place, where a block moves a single 16-byte column, half a sector, so
+// that all SMs have one. 24 sequences of 900 to 9000 rows, 2000 kept: 55 us
+// either way (26 us are the bytes: the weights once, each kept row once each
+// way).
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -18,11 +18,11 @@
 // cosines, once for all its heads: angle reduced to half turns in FP64 (at
 // position 10^5 an FP32 product is off by 2^-8 of a radian), sine and cosine
 // of the remainder in FP32.
-// Measured: 12868 bf16 rows of 32 + 2 x 8 heads of 64 43.5 us (3.6 TB/s; the bytes
-// alone are 24 us). Issue slots are 63 % busy, the ALU 54 %, DRAM 31 %: warps
-// wait for fixed latencies and global loads about as long as they work, and the
-// partner half of a head is shuffled raw and unpacked a second time. 8 rows
-// 3.8 us.
+// Measured: 12868 bf16 rows of 32 + 2 x 8 heads of 64 43.5 us (3.6 TB/s; the
+// bytes alone are 24 us). Issue slots are 63 % busy, the ALU 54 %, DRAM 31 %:
+// warps wait for fixed latencies and global loads about as long as they work,
+// and the partner half of a head is shuffled raw and unpacked a second time. 8
+// rows 3.8 us.
 #include <algorithm>
 
 #include "kernels.cuh"

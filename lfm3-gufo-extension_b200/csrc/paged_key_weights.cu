@@ -14,13 +14,14 @@
 // half of tensor memory while the other half is computed. One exponential per
 // (key, column) is the bound for chunks, reading K for single tokens (columns
 // are then a multiple of 16). Blocks take equal shares of (key pair, KV head,
-// column block) units (paged_plan.cuh); sums run in the order of units, then
-// of blocks. Measured: 512 bf16 rows at depth 8192 (69 M exponentials, 15 us
-// of the special function units) 43.6 us for the three kernels (`sums` waits for
+// column block) units (paged_plan.cuh); sums run in the order of units, then of
+// blocks. Measured: 512 bf16 rows at depth 8192 (69 M exponentials, 15 us of
+// the special function units) 43.6 us for the three kernels (`sums` waits for
 // tensor memory: the special function units are busy for 44 %, issue slots for
 // 24 % of it); 16 FP32 single tokens over 1024 to 8192 keys 19 us, K at 3.6
-// TB/s. A polynomial on the FMA pipe for a quarter of the exponentials was no faster (45 us: the choice
-// between the two costs what it saves), nor were 64 columns a read (43.6 us).
+// TB/s. A polynomial on the FMA pipe for a quarter of the exponentials was no
+// faster (45 us: the choice between the two costs what it saves), nor were 64
+// columns a read (43.6 us).
 // Warps: 8 TMA, 9 tensor memory and MMA, 10 the columns' factors, 11 segments.
 #include <algorithm>
 #include <type_traits>

@@ -340,17 +340,16 @@ struct ChunkSegment {
 // short stretches (4 of 2000 rows: 279 us without the places, 144 us with).
 // With more stretches than blocks, blocks may take whole ones instead, the same
 // number each: that is no slower when they are about as long (chunks under a
-// window of 256: 53 us crossing, 50.5 us whole), since nothing has to be merged.
-// (24 chunks of 30 to 40 rows at 100 to 300 keys show the estimate's limits: 38 us
-// whole, as it says, 35 us crossing.)
-// With fewer, the smallest share with which rounded stretches still fit the
-// blocks is taken, unless crossing shares save more than a second segment
-// costs. That is worth 15 % where stretches are few and short (1024 f16 rows at
-// depth 1000 48 us padded, 56 us crossing) and costs up to 4 % where they are
-// long (512 FP32 rows at depth 8192, 32 stretches of 65 to 68 tiles, shares of 17
-// tiles instead of 15: 91 us padded, 88 us crossing) and 17 % for 200 f16 rows
-// from position 0 (23 and 19 us); over 72 batches of 1 to 4 chunks the two are
-// within 1 %.
+// window of 256: 53 us crossing, 50.5 us whole), since nothing has to be
+// merged. (24 chunks of 30 to 40 rows at 100 to 300 keys show the estimate's
+// limits: 38 us whole, as it says, 35 us crossing.) With fewer, the smallest
+// share with which rounded stretches still fit the blocks is taken, unless
+// crossing shares save more than a second segment costs. That is worth 15 %
+// where stretches are few and short (1024 f16 rows at depth 1000 48 us padded,
+// 56 us crossing) and costs up to 4 % where they are long (512 FP32 rows at
+// depth 8192, 32 stretches of 65 to 68 tiles, shares of 17 tiles instead of 15:
+// 91 us padded, 88 us crossing) and 17 % for 200 f16 rows from position 0 (23
+// and 19 us); over 72 batches of 1 to 4 chunks the two are within 1 %.
 __device__ inline int64_t chunk_plan(PagedLine<ChunkUnits>& line) {
   const PagedTables& t = line.t;
   const ChunkUnits& units = line.units;
