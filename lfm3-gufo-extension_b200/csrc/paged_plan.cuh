@@ -349,7 +349,7 @@ struct ChunkSegment {
 // 56 us crossing) and costs up to 4 % where they are long (512 FP32 rows at
 // depth 8192, 32 stretches of 65 to 68 tiles, shares of 17 tiles instead of 15:
 // 91 us padded, 88 us crossing) and 17 % for 200 f16 rows from position 0 (23
-// and 19 us); over 72 batches of 1 to 4 chunks the two are within 1 %.
+// and 19 us); over 72 batches of 1 to 4 chunks it costs 1 % on average.
 __device__ inline int64_t chunk_plan(PagedLine<ChunkUnits>& line) {
   const PagedTables& t = line.t;
   const ChunkUnits& units = line.units;
