@@ -346,7 +346,7 @@ struct ChunkSegment {
 // share with which rounded stretches still fit the blocks is taken, unless
 // crossing shares save more than a second segment costs. That is worth 15 %
 // where stretches are few and short (1024 f16 rows at depth 1000 48 us padded,
-// 56 us crossing) and costs up to 4 % where they are long (512 FP32 rows at
+// 56 us crossing) and costs up to 5 % where they are long (512 FP32 rows at
 // depth 8192, 32 stretches of 65 to 68 tiles, shares of 17 tiles instead of 15:
 // 91 us padded, 88 us crossing) and 17 % for 200 f16 rows from position 0 (23
 // and 19 us); over 72 batches of 1 to 4 chunks it costs 1 % on average.
